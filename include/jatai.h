@@ -188,6 +188,30 @@ int jt_atencao_ws_qs(const void* qm, const void* qE, void* Om, void* OE, void* P
 int jt_atencao_back_ws_qs(const void* gom, const void* goE, const void* qm, const void* qE, const void* P, void* Gm, void* GE, int Bt, int T,
                           int H, int D, int GA, int limite, void* ws, long long ws_bytes, const void* salvo, long long salvo_bytes, int kid);
 
+/* ---- generation (no reference counterpart: the reference only trains). A paged cache of keys and values: m int8
+ * [npag][camadas][2: keys, values][Hk][pag][hd], E int8 [npag][camadas][2][Hk][pag][hd / min(hd, BLK)]; hd 4, 16, 32, 64
+ * or 128, pag a power of two from 16 to 1024. A token at position j of sequence b is slot j % pag of page tab[b][j / pag].
+ * Rows: a block tensor qm int8 [M, (H + 2 Hk) hd], qE; sequence b's newest tokens are the rows ini[b] .. ini[b + 1] - 1
+ * (ini null: row b), at positions comp[b] - (ini[b + 1] - ini[b]) .. comp[b] - 1. tab int32 [B][P], comp int32 [B], ini
+ * int32 [B + 1] are device arrays read by the kernels; novos and teto (<= P pag) bound a sequence's rows and comp. A
+ * sequence outside those bounds and a page outside 0 .. npag - 1 that a row needs raise E_ARG; neither is read. */
+int jt_cache_grava(const void* qm, const void* qE, void* cm, void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag,
+                   const void* tab, const void* comp, const void* ini, int M, int B, int P, int novos, int teto, int H, int kid);
+/* pares: HOST array of n (source, target) int pages, copied over all layers; hipErrorInvalidValue where a target repeats, is
+ * a source, or a page is outside the cache */
+int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, int pag, const void* pares, int n, int kid);
+/* out [M, H hd]: softmax_j(q . k_j / sqrt(hd) - incl[h] (i - j)) . v_j over the visible tokens j <= i of the row's sequence:
+ * all (janela 0), or the last janela and the first sumid. Query head h reads head h / (H / Hk); incl float [H] or null.
+ * tipo 0: block tensor (out int8, outE), 1: bfloat16, 2: fp32. Rows of no sequence come out as zeros. ws: workspace of
+ * jt_atencao_cache_ws_bytes bytes, 16-byte aligned, not shared by calls that overlap. */
+long long jt_atencao_cache_ws_bytes(int M, int H, int hd, int teto, int janela, int sumid);
+int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag,
+                     const void* tab, const void* comp, const void* ini, const void* incl, void* out, void* outE, int M, int B, int P,
+                     int novos, int teto, int H, int janela, int sumid, int tipo, void* ws, long long ws_bytes, int kid);
+/* the values of a block tensor (cru 0: m int8, E int8 per block) or a raw one (cru 1: int32, int16 per value) of n values, as
+ * bfloat16 (tipo 1, block tensors only) or fp32 (tipo 2), each rounded once */
+int jt_valores(const void* m, const void* E, void* out, long long n, int cru, int tipo, int kid);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,7 @@
 #include "jt_atencao.hip"
 #include "jt_atencao_hd.hip"
 #include "jt_atencao_ws.hip"
+#include "jt_cache.hip"
 
 __device__ Erro g_erro;
 // A host-pinned flag beside the record (set up by the first jt_erro_le): 1 once an event is recorded, 0 after each
@@ -975,4 +976,136 @@ int jt_atencao_back_ws_qs(const void* gom, const void* goE, const void* qm, cons
     return atencao_back_ws(gom, goE, qm, qE, P, Gm, GE, Bt, T, H, D, GA, limite, ws, ws_bytes, true, kid, salvo);
 }
 
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------- paged cache
+// No reference counterpart (the reference only trains): keys and values of a model that answers, kept in pages.
+// Cache shape: m int8 [npag][camadas][2][Hk][pag][hd], E int8 [npag][camadas][2][Hk][pag][hd / min(hd, BLK)].
+static bool cache_ok(const void* cm, const void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag) {
+    return cm && cE && alinhados(cm, cE) && npag > 0 && camadas > 0 && camada >= 0 && camada < camadas && Hk > 0 && Hk <= 4096 &&
+           (hd == 4 || hd == 16 || hd == 32 || hd == 64 || hd == 128) && pag >= 16 && pag <= 1024 && (pag & (pag - 1)) == 0 &&
+           2LL * camadas * Hk * pag * hd < (1LL << 40);
+}
+static bool lote_ok(const void* tab, const void* comp, int M, int B, int P, int pag, int novos, int teto) {
+    return tab && comp && M >= 0 && B > 0 && P > 0 && novos >= 0 && teto >= 0 && teto <= (1 << 30) && teto <= (long long)P * pag;
+}
+static int grupos(int hd) { return hd / std::min(hd, g_blk); }
+// calls F(hd, values per exponent of a head) for the cache's head width and block size
+#define POR_CABECA(F)                                                                                                              \
+    switch (hd) {                                                                                                                  \
+        case 4: F(4, 4); break;                                                                                                    \
+        case 16: F(16, 16); break;                                                                                                 \
+        case 32: F(32, 32); break;                                                                                                 \
+        case 64: if (g_blk == 32) F(64, 32); else F(64, 64); break;                                                                \
+        default: if (g_blk == 32) F(128, 32); else F(128, 128);                                                                    \
+    }
+extern "C" {
+int jt_cache_grava(const void* qm, const void* qE, void* cm, void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag,
+                   const void* tab, const void* comp, const void* ini, int M, int B, int P, int novos, int teto, int H, int kid) {
+    if (!cache_ok(cm, cE, npag, camadas, camada, Hk, hd, pag) || !lote_ok(tab, comp, M, B, P, pag, novos, teto)) return (int)hipErrorInvalidValue;
+    if (M == 0) return 0;
+    if (!qm || !qE || !alinhado(qm) || H < 0 || H > 65535 || (long long)(H + 2LL * Hk) * hd % g_blk) return (int)hipErrorInvalidValue;
+    const atc::Lote L{(const int*)tab, (const int*)comp, (const int*)ini, B, P, M, ilog2(pag), npag, novos, teto};
+    const long long camada_m = 2LL * Hk * pag * hd, camada_e = 2LL * Hk * pag * grupos(hd);
+    const int rpw = hd <= 16 ? 64 : 1024 / hd;                        // rows per wave
+    const dim3 grade((M + rpw - 1) / rpw, (2 * Hk + 3) / 4);
+#define F(HD, GS) (k_cache_grava<HD, GS><<<grade, 256, 0, g_stream>>>((const int8_t*)qm, (const int8_t*)qE, (int8_t*)cm + camada * camada_m, \
+                   (int8_t*)cE + camada * camada_e, L, H, Hk, ilog2(g_blk), camadas * camada_m, camadas * camada_e, kid))
+    POR_CABECA(F)
+#undef F
+    return fim();
+}
+
+// pares: HOST array of n (source, target) pages. Targets that repeat, or that are some pair's source, are refused: the
+// copies run side by side.
+int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, int pag, const void* pares, int n, int kid) {
+    (void)kid;
+    if (!cache_ok(cm, cE, npag, camadas, 0, Hk, hd, pag) || n < 0 || (n > 0 && !pares)) return (int)hipErrorInvalidValue;
+    if (n == 0) return 0;
+    const int* x = (const int*)pares;
+    unsigned char* marca = (unsigned char*)calloc((size_t)npag, 1);    // 1: source, 2: target
+    if (!marca) return (int)hipErrorOutOfMemory;
+    bool ok = true;
+    for (int i = 0; i < 2 * n && ok; i++) ok = x[i] >= 0 && x[i] < npag;
+    for (int i = 0; i < n && ok; i++) marca[x[2 * i]] = 1;
+    for (int i = 0; i < n && ok; i++) { ok = marca[x[2 * i + 1]] == 0; marca[x[2 * i + 1]] = 2; }
+    free(marca);
+    if (!ok) return (int)hipErrorInvalidValue;
+    const long long pag_m = 2LL * camadas * Hk * pag * hd, pag_e = 2LL * camadas * Hk * pag * grupos(hd);
+    for (int base = 0; base < n; base += PARES_COPIA) {
+        ParesCopia ps;
+        const int k = std::min(PARES_COPIA, n - base);
+        for (int i = 0; i < k; i++) { ps.de[i] = x[2 * (base + i)]; ps.para[i] = x[2 * (base + i) + 1]; }
+        const long long wg = ((pag_m + pag_e) / 16 + 255) / 256;
+        k_cache_copia<<<dim3((unsigned)std::min(wg, 1024LL), k), 256, 0, g_stream>>>((int8_t*)cm, (int8_t*)cE, ps, pag_m, pag_e);
+        const int rc = fim();
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+// Splits of a row's visible tokens, and tokens per split: as many as fill the chip (8 workgroups of 4 waves per CU), each with
+// at least one step of a workgroup's loop (256 tokens at head width 64).
+static void atc_divide(long long M, int H, int hd, int teto, int janela, int sumid, int& S, int& fatia) {
+    const long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto);
+    const long long passo = hd <= 16 ? 1024 : 16384 / hd, max_s = (nv + passo - 1) / passo;
+    const long long s = std::min(std::max(2048 / std::max(M * H, 1LL), 1LL), max_s);
+    fatia = (int)(((nv + s - 1) / s + passo - 1) / passo * passo);
+    S = (int)((nv + fatia - 1) / fatia);
+}
+long long jt_atencao_cache_ws_bytes(int M, int H, int hd, int teto, int janela, int sumid) {
+    if (M <= 0 || H <= 0 || hd <= 0 || teto < 0 || teto > (1 << 30)) return 0;
+    int S, fatia;
+    atc_divide(M, H, hd, teto, janela, sumid, S, fatia);
+    return (long long)M * H * S * (hd + 2) * 4 + 16;
+}
+int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag,
+                     const void* tab, const void* comp, const void* ini, const void* incl, void* out, void* outE, int M, int B, int P,
+                     int novos, int teto, int H, int janela, int sumid, int tipo, void* ws, long long ws_bytes, int kid) {
+    if (!cache_ok(cm, cE, npag, camadas, camada, Hk, hd, pag) || !lote_ok(tab, comp, M, B, P, pag, novos, teto)) return (int)hipErrorInvalidValue;
+    if (M == 0) return 0;
+    if (!qm || !qE || !out || !alinhados(qm, out, ws) || H <= 0 || H > 65535 || H % Hk || (long long)(H + 2LL * Hk) * hd % g_blk) return (int)hipErrorInvalidValue;
+    if (janela < 0 || sumid < 0 || tipo < 0 || tipo > 2 || (tipo == 0 && (!outE || H * hd % g_blk))) return (int)hipErrorInvalidValue;
+    if (!ws || ws_bytes < jt_atencao_cache_ws_bytes(M, H, hd, teto, janela, sumid)) return (int)hipErrorInvalidValue;
+    int S, fatia;
+    atc_divide(M, H, hd, teto, janela, sumid, S, fatia);
+    const long long camada_m = 2LL * Hk * pag * hd, camada_e = 2LL * Hk * pag * grupos(hd), partes = (long long)M * H * S;
+    float *ml = (float*)ws, *po = ml + (2 * partes + 3) / 4 * 4;
+    const atc::Args a{(const int8_t*)qm, (const int8_t*)qE, (const int8_t*)cm + camada * camada_m, (const int8_t*)cE + camada * camada_e,
+                      (const float*)incl, ml, po, camadas * camada_m, camadas * camada_e,
+                      atc::Lote{(const int*)tab, (const int*)comp, (const int*)ini, B, P, M, ilog2(pag), npag, novos, teto},
+                      H, Hk, ilog2(g_blk), janela, sumid, S, fatia, kid};
+#define F(HD, GS) (k_atc_um<HD, GS><<<dim3(M, H, S), 256, 0, g_stream>>>(a))
+    POR_CABECA(F)
+#undef F
+    int rc = fim();
+    if (rc) return rc;
+    const int C = H * hd;
+    const dim3 grade(M, (C + 1023) / 1024);
+#define J(BL, T) (k_atc_junta<BL, T><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, S, kid))
+    if (tipo == 1) J(32, 1);
+    else if (tipo == 2) J(32, 2);
+    else if (g_blk == 32) J(32, 0);
+    else J(128, 0);
+#undef J
+    return fim();
+}
+
+// ---------------------------------------------------------------------------------------------- values as floats
+// m int8 and E int8 per block (cru 0), or int32 and int16 per value (cru 1, n values), to bfloat16 (tipo 1; cru 0 only) or fp32 (2)
+int jt_valores(const void* m, const void* E, void* out, long long n, int cru, int tipo, int kid) {
+    (void)kid;
+    if (n <= 0) return n == 0 ? 0 : (int)hipErrorInvalidValue;
+    if (!m || !E || !out || !alinhados(m, E, out) || (cru != 0 && cru != 1) || (tipo != 2 && (tipo != 1 || cru))) return (int)hipErrorInvalidValue;
+    if (cru) {
+        if ((n + 255) / 256 > 0x7fffffff) return (int)hipErrorInvalidValue;
+        k_valores_cru<<<(unsigned)((n + 255) / 256), 256, 0, g_stream>>>((const int*)m, (const int16_t*)E, (float*)out, n);
+        return fim();
+    }
+    if (n % g_blk || (n + 2047) / 2048 > 0x7fffffff) return (int)hipErrorInvalidValue;
+    const unsigned wg = (unsigned)((n + 2047) / 2048);
+    if (tipo == 1) k_valores<1><<<wg, 256, 0, g_stream>>>((const int8_t*)m, (const int8_t*)E, out, n, ilog2(g_blk));
+    else k_valores<2><<<wg, 256, 0, g_stream>>>((const int8_t*)m, (const int8_t*)E, out, n, ilog2(g_blk));
+    return fim();
+}
 }  // extern "C"

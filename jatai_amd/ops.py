@@ -14,6 +14,7 @@ There is no CPU fallback: if libjatai.so is missing or fails to load, constructi
 import ctypes
 import math
 import os
+import typing
 
 import torch
 
@@ -35,7 +36,8 @@ FUNCOES = ("jt_gemm", "jt_gemm_f", "jt_quant", "jt_soma", "jt_relu2", "jt_relu2_
            "jt_atencao_ws", "jt_atencao_back_ws", "jt_gemm_lote", "jt_entrada_g_bytes",
            "jt_gemm_otim_lote", "jt_entrada_go_bytes", "jt_atencao_ws_q", "jt_atencao_back_ws_q",
            "jt_rms_back_soma", "jt_perda", "jt_gemm_tile", "jt_gemm_tile_k", "jt_gemm_soma16", "jt_rms_back_soma16", "jt_atencao_ws_qs",
-           "jt_atencao_back_ws_qs", "jt_janelas", "jt_otimizador_t")
+           "jt_atencao_back_ws_qs", "jt_janelas", "jt_otimizador_t", "jt_cache_grava", "jt_cache_copia", "jt_atencao_cache",
+           "jt_valores")
 VOIDS = ("jt_stream", "jt_gemm_split", "jt_gemm_bm", "jt_atencao_linhas", "jt_atencao_mfma")
 
 
@@ -60,7 +62,20 @@ def carrega_lib(caminho=LIB):
     lib.jt_atencao_ws_bytes.restype = ctypes.c_longlong
     lib.jt_atencao_back_ws_bytes.restype = ctypes.c_longlong
     lib.jt_atencao_salvo_bytes.restype = ctypes.c_longlong
+    lib.jt_atencao_cache_ws_bytes.restype = ctypes.c_longlong
     return lib
+
+
+class Lote(typing.NamedTuple):
+    """The sequences of one generation call. tabela int32 [B, P]: the cache page of each run of slots (-1: none); comp
+    int32 [B]: tokens of each sequence, the new ones among them; ini int32 [B + 1]: first row of each sequence's new
+    tokens, and the end of the last's (None: row b is sequence b's one new token). novos and teto bound, on the host,
+    the new tokens of a sequence and comp; the tensors are read when the kernels run, so a captured graph follows them."""
+    tabela: torch.Tensor
+    comp: torch.Tensor
+    ini: torch.Tensor
+    novos: int
+    teto: int
 
 
 class OpsHip:
@@ -90,6 +105,8 @@ class OpsHip:
             return NULO
         if isinstance(x, int):
             return ctypes.c_longlong(x) if abs(x) > 2**31 - 1 else x
+        if isinstance(x, ctypes.Array):             # a host array: its address
+            return ctypes.cast(x, ctypes.c_void_p)
         return ctypes.c_int(x)
 
     # A launch's host path is what bounds an op-by-op step of small tensors, so it makes no object and formats no
@@ -685,3 +702,97 @@ class OpsHip:
         n = W[0].numel() // BLK
         self._lanca("peso", "jt_peso", (W[0], W[1], Mom[0], Mom[1], R[0], R[1], k, int(ef), n), dict(), tuple(W[0].shape), longos=(8,))
         return W, R
+
+    # ---------------------------------------------------------------- generation: the paged cache (no reference counterpart)
+    # A cache is the pair (m int8 [pages, layers, 2, Hk, pag, hd], E int8 [pages, layers, 2, Hk, pag, hd / min(hd, BLK)]):
+    # keys and values of Hk heads of width hd, as the Q/K/V product wrote them. jatai_amd.cache.CacheKV keeps one.
+    def _confere_cache(self, op, C):
+        m, E = C
+        f = m.shape
+        if not (m.dtype == torch.int8 and E.dtype == torch.int8 and m.is_cuda and E.is_cuda and m.dim() == 6 and m.is_contiguous()
+                and E.is_contiguous() and f[2] == 2 and f[5] in (4, 16, 32, 64, 128) and f[4] in (16, 32, 64, 128, 256, 512, 1024)
+                and E.shape == (*f[:5], f[5] // min(f[5], BLK)) and m.numel() and m.get_device() == torch.cuda.current_device()):
+            self.reg.falha(f"{op}: cache {tuple(f)} {m.dtype} / {tuple(E.shape)} {E.dtype}: esperados int8 contiguos [paginas, camadas, 2, Hk, "
+                           f"pagina, hd] e [.., hd / min(hd, {BLK})] na GPU atual, pagina potencia de 2 de 16 a 1024, hd 4, 16, 32, 64 ou 128")
+        return f
+
+    def _confere_lote(self, op, QKV, C, camada, lote):
+        """The shapes of a call over the cache: (pages, layers, Hk, hd, slots, H, B, P)."""
+        paginas, camadas, _, Hk, pag, hd = self._confere_cache(op, C)
+        self.reg.confere_bloco("qkv", QKV)
+        m = QKV[0]
+        H = m.shape[1] // hd - 2 * Hk
+        if not (m.shape[1] == (H + 2 * Hk) * hd and H > 0 and H % Hk == 0 and 0 <= camada < camadas and m.get_device() == C[0].get_device()):
+            self.reg.falha(f"{op}: qkv {tuple(m.shape)}, camada {camada} de {camadas}, {Hk} cabecas de {hd} no cache")
+        tab, comp, ini = lote.tabela, lote.comp, lote.ini
+        B = comp.shape[0] if comp.dim() == 1 else -1
+        for n, t, f in (("tabela", tab, (B, tab.shape[-1])), ("comp", comp, (B,))) + ((("ini", ini, (B + 1,)),) if ini is not None else ()):
+            if not (t.dtype == torch.int32 and t.is_contiguous() and t.shape == f and t.is_cuda and t.get_device() == m.get_device() and t.numel()):
+                self.reg.falha(f"{op}: {n} {tuple(t.shape)} {t.dtype}, esperado int32 {f} contiguo na GPU de qkv")
+        if not (0 <= lote.novos <= 2**30 and 0 <= lote.teto <= min(2**30, tab.shape[1] * pag)):
+            self.reg.falha(f"{op}: novos={lote.novos}, teto={lote.teto} para {tab.shape[1]} paginas de {pag}")
+        return paginas, camadas, Hk, hd, pag, H, B, tab.shape[1]
+
+    def cache_grava(self, QKV, C, camada, lote):
+        """The keys and values of every new row of the block tensor QKV [M, (H + 2 Hk) hd] into the slots of their
+        positions, in place; returns C. Rows that belong to no sequence write nothing. Two sequences of a call must not
+        share the pages that they write."""
+        paginas, camadas, Hk, hd, pag, H, B, P = self._confere_lote("cache_grava", QKV, C, camada, lote)
+        M = QKV[0].shape[0]
+        self._lanca("cache_grava", "jt_cache_grava", (*QKV, *C, paginas, camadas, camada, Hk, hd, pag, lote.tabela, lote.comp, lote.ini, M, B, P,
+                                                      lote.novos, lote.teto, H), dict(qkv=QKV[0], tabela=lote.tabela, comp=lote.comp), (M, H + 2 * Hk))
+        return C
+
+    def cache_copia(self, C, pares):
+        """Pages copied within the cache, every layer of them, in place; returns C. pares: [(source, target)], the targets
+        distinct and none of them a source."""
+        paginas, camadas, _, Hk, pag, hd = self._confere_cache("cache_copia", C)
+        v = [p for par in pares for p in par]
+        if not (len(v) == 2 * len(pares) and all(0 <= p < paginas for p in v) and len({*v[1::2]}) == len(pares) and not {*v[1::2]} & {*v[::2]}):
+            self.reg.falha(f"cache_copia: pares (origem, destino) de paginas 0 a {paginas - 1}, destinos distintos e nenhum deles origem; recebeu {pares}")
+        tab = (ctypes.c_int * len(v))(*v)
+        self._lanca("cache_copia", "jt_cache_copia", (*C, paginas, camadas, Hk, hd, pag, tab, len(pares)), dict(), (len(pares),))
+        return C
+
+    def atencao_cache(self, QKV, C, camada, lote, incl=None, janela=0, sumidouros=0, saida=None):
+        """Attention of the new rows of QKV [M, (H + 2 Hk) hd] (queries in its first H hd columns) over the cache, whose
+        slots already hold their own keys and values (cache_grava). Query head h reads head h // (H / Hk). A row at position i sees
+        the tokens j <= i of its sequence; with janela > 0 the last `janela` of them and the first `sumidouros`:
+            softmax_j(q . k_j / sqrt(hd) - incl[h] (i - j)) . v_j,  incl float32 [H] or None (see inclinacoes)
+        Products are exact, statistics float32. Returns a block tensor [M, H hd] (saida None) or a torch.bfloat16 or
+        torch.float32 tensor, rounded once; rows that belong to no sequence come out as zeros."""
+        paginas, camadas, Hk, hd, pag, H, B, P = self._confere_lote("atencao_cache", QKV, C, camada, lote)
+        m, E = QKV
+        M, D = m.shape[0], H * hd
+        if incl is not None and not (incl.dtype == torch.float32 and incl.shape == (H,) and incl.is_contiguous() and incl.is_cuda
+                                     and incl.get_device() == m.get_device()):
+            self.reg.falha(f"atencao_cache: incl {tuple(incl.shape)} {incl.dtype}, esperado float32 {(H,)} na GPU de qkv")
+        if not (saida in (None, torch.bfloat16, torch.float32) and 0 <= janela <= 2**30 and 0 <= sumidouros <= 2**30 and (saida is not None or D % BLK == 0)):
+            self.reg.falha(f"atencao_cache: janela={janela}, sumidouros={sumidouros}, saida={saida} (None com H hd multiplo de {BLK}, bfloat16 ou float32)")
+        Y = self._novo_bloco(M, D, m.device) if saida is None else (torch.empty(M, D, dtype=saida, device=m.device), None)
+        nws = self.lib.jt_atencao_cache_ws_bytes(M, H, hd, lote.teto, janela, sumidouros)
+        ws = torch.empty(nws, dtype=torch.uint8, device=m.device)
+        self._lanca("atencao_cache", "jt_atencao_cache",
+                    (m, E, *C, paginas, camadas, camada, Hk, hd, pag, lote.tabela, lote.comp, lote.ini, incl, *Y, M, B, P, lote.novos, lote.teto, H,
+                     janela, sumidouros, {None: 0, torch.bfloat16: 1, torch.float32: 2}[saida], ws, nws),
+                    dict(qkv=m, qkvE=E, tabela=lote.tabela, comp=lote.comp), (M, D), longos=(26,))
+        return Y if saida is None else Y[0]
+
+    @staticmethod
+    def inclinacoes(H, hd, dev="cuda"):
+        """The training attention's position bias per head, in nats per token of distance (float32 [H]): 2^(incl - 8) with
+        incl = 8 - h // 8 at head width 4 (ops.py:205; 0 once incl is negative) and 8 - (8 h) // H at other widths."""
+        incl = [8 - h // 8 if hd == 4 else 8 - 8 * h // H for h in range(H)]
+        return torch.tensor([2.0 ** (i - 8) if i >= 0 else 0.0 for i in incl], dtype=torch.float32, device=dev)
+
+    def valores(self, X, tipo=torch.float32):
+        """The values of a block tensor (tipo torch.float32 or torch.bfloat16, exact in both) or of a raw tensor (float32,
+        rounded once): what de_f32 is the inverse of."""
+        m, E = X
+        cru = m.dtype == torch.int32
+        (self.reg.confere_cru if cru else self.reg.confere_bloco)("x", X)
+        if not (tipo == torch.float32 or (tipo == torch.bfloat16 and not cru)):
+            self.reg.falha(f"valores: tipo {tipo} (float32; bfloat16 para tensores em blocos)")
+        y = torch.empty(m.shape, dtype=tipo, device=m.device)
+        self._lanca("valores", "jt_valores", (m, E, y, m.numel(), int(cru), 1 if tipo == torch.bfloat16 else 2), dict(m=m, E=E), tuple(m.shape), longos=(3,))
+        return y
