@@ -211,6 +211,16 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
 /* the values of a block tensor (cru 0: m int8, E int8 per block) or a raw one (cru 1: int32, int16 per value) of n values, as
  * bfloat16 (tipo 1, block tensors only) or fp32 (tipo 2), each rounded once */
 int jt_valores(const void* m, const void* E, void* out, long long n, int cru, int tipo, int kid);
+/* Products of a few rows with 4-bit weights W [N, K] = q s 2^eb, q in [-7, 7], a scale per row and block of BLK columns.
+ * Packed form: w4 uint8 [ceil(N/16)][ceil(K/128)][64][16], byte 4 a + i of lane l = row l % 16's columns 32 a + 8 (l / 16) + i
+ * (low four bits, two's complement) and + 4 (high); esc bfloat16 [ceil(N/16)][ceil(K/128)][16][128 / BLK] = s 2^(eb - R);
+ * R int16 [N], the row's largest eb; K a multiple of BLK up to 256 BLK. jt_para4 packs a block tensor (once per weight).
+ * jt_gemv4: acc_ij = sum over blocks of rnd(p s 2^(eb - R_j) 2^(ea - RA_i) 2^-g), half to even, exponent RA_i + R_j + g, with p
+ * the exact dot product, ea and RA_i x's exponents and their row maximum, g = log2(BLK) - 4. modo 1: raw (y int32, yE int16
+ * [M, N], any N); 0: quantized to a block tensor (N % BLK == 0); 2: jt_soma of that with res, resE; 3: jt_relu2 of it. */
+int jt_para4(const void* m, const void* E, void* w4, void* esc, void* R, int N, int K, int kid);
+int jt_gemv4(const void* x, const void* xE, const void* w4, const void* esc, const void* R, const void* res, const void* resE, void* y, void* yE,
+             int M, int N, int K, int modo, int kid);
 
 #ifdef __cplusplus
 }

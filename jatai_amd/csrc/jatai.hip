@@ -19,6 +19,7 @@
 #include "jt_atencao_hd.hip"
 #include "jt_atencao_ws.hip"
 #include "jt_cache.hip"
+#include "jt_gemv4.hip"
 
 __device__ Erro g_erro;
 // A host-pinned flag beside the record (set up by the first jt_erro_le): 1 once an event is recorded, 0 after each
@@ -1106,6 +1107,41 @@ int jt_valores(const void* m, const void* E, void* out, long long n, int cru, in
     const unsigned wg = (unsigned)((n + 2047) / 2048);
     if (tipo == 1) k_valores<1><<<wg, 256, 0, g_stream>>>((const int8_t*)m, (const int8_t*)E, out, n, ilog2(g_blk));
     else k_valores<2><<<wg, 256, 0, g_stream>>>((const int8_t*)m, (const int8_t*)E, out, n, ilog2(g_blk));
+    return fim();
+}
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------- 4-bit weights
+extern "C" {
+// w4 uint8 [ceil(N / 16)][ceil(K / 128)][64][16], esc bf16 [ceil(N / 16)][ceil(K / 128)][16][128 / BLK], R int16 [N]
+int jt_para4(const void* m, const void* E, void* w4, void* esc, void* R, int N, int K, int kid) {
+    (void)kid;
+    if (N <= 0 || K <= 0 || K % g_blk || K > 256 * g_blk || !m || !E || !w4 || !esc || !R || !alinhados(m, w4, esc, R)) return (int)hipErrorInvalidValue;
+#define C(BL) (k_para4<BL><<<(N + 15) / 16, 256, 0, g_stream>>>((const int8_t*)m, (const int8_t*)E, (int8_t*)w4, (uint16_t*)esc, (int16_t*)R, N, K), 0)
+    POR_BLK(C);
+#undef C
+    return fim();
+}
+// modo 0: y int8 [M, N], yE int8 [M, N / BLK] | 1: y int32, yE int16 [M, N] (any N) | 2: block sum with the residual res, resE
+// | 3: block relu^2 of the block product
+int jt_gemv4(const void* x, const void* xE, const void* w4, const void* esc, const void* R, const void* res, const void* resE, void* y, void* yE,
+             int M, int N, int K, int modo, int kid) {
+    using namespace gv4;
+    if (M < 0 || N <= 0 || K <= 0 || K % g_blk || K > 256 * g_blk || modo < 0 || modo > 3 || (modo != 1 && N % g_blk)) return (int)hipErrorInvalidValue;
+    if (M == 0) return 0;
+    if (!x || !xE || !w4 || !esc || !R || !y || !yE || !alinhados(x, w4, esc, R, y, yE) || (modo == 2 && (!res || !resE || !alinhado(res)))) return (int)hipErrorInvalidValue;
+    const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4, Kt = (K + 127) / 128, cg = modo == 1 ? 1 : g_blk / COLS, ks = std::min(Kt, (mt == 4 ? 8 : 16) / cg);
+    const Args a{(const int8_t*)x, (const int8_t*)xE, (const int4*)w4, (const uint16_t*)esc, (const int16_t*)R, (const int8_t*)res, (const int8_t*)resE,
+                 y, yE, M, N, K, modo, ks, cg, kid};
+    const dim3 grade((N + COLS * cg - 1) / (COLS * cg), (M + 16 * mt - 1) / (16 * mt));
+    if (grade.y > 65535) return (int)hipErrorInvalidValue;
+    const size_t lds = 4 * ((size_t)K / g_blk * 16 * mt + 16 * mt + (size_t)16 * mt * COLS * cg);
+#define L(BL, NR, MT) (lds_max(k_gemv4<BL, NR, MT>, lds), k_gemv4<BL, NR, MT><<<grade, 64 * ks * cg, lds, g_stream>>>(a))
+#define LM(BL) (M <= 4 ? L(BL, 1, 1) : M <= 8 ? L(BL, 2, 1) : M <= 16 ? L(BL, 4, 1) : M <= 32 ? L(BL, 4, 2) : L(BL, 4, 4))
+    if (g_blk == 32) LM(32);
+    else LM(128);
+#undef LM
+#undef L
     return fim();
 }
 }  // extern "C"

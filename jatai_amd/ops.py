@@ -37,7 +37,7 @@ FUNCOES = ("jt_gemm", "jt_gemm_f", "jt_quant", "jt_soma", "jt_relu2", "jt_relu2_
            "jt_gemm_otim_lote", "jt_entrada_go_bytes", "jt_atencao_ws_q", "jt_atencao_back_ws_q",
            "jt_rms_back_soma", "jt_perda", "jt_gemm_tile", "jt_gemm_tile_k", "jt_gemm_soma16", "jt_rms_back_soma16", "jt_atencao_ws_qs",
            "jt_atencao_back_ws_qs", "jt_janelas", "jt_otimizador_t", "jt_cache_grava", "jt_cache_copia", "jt_atencao_cache",
-           "jt_valores")
+           "jt_valores", "jt_para4", "jt_gemv4")
 VOIDS = ("jt_stream", "jt_gemm_split", "jt_gemm_bm", "jt_atencao_linhas", "jt_atencao_mfma")
 
 
@@ -796,3 +796,55 @@ class OpsHip:
         y = torch.empty(m.shape, dtype=tipo, device=m.device)
         self._lanca("valores", "jt_valores", (m, E, y, m.numel(), int(cru), 1 if tipo == torch.bfloat16 else 2), dict(m=m, E=E), tuple(m.shape), longos=(3,))
         return y
+
+    # ---------------------------------------------------------------- generation: 4-bit weights (no reference counterpart)
+    def para4(self, W):
+        """A block tensor W [N, K] packed to 4 bits a weight, with one scale per row and block, once: (uint8 [ceil(N / 16),
+        ceil(K / 128), 64, 16], bfloat16 [ceil(N / 16), ceil(K / 128), 16, 128 / BLK], int16 [N]), what gemv4 takes. A weight
+        becomes the nearest of 15 values spaced by a seventh of its block's largest."""
+        self.reg.confere_bloco("W", W)
+        m, E = W
+        N, K = m.shape
+        self.reg.exige(0 < K <= 256 * BLK and N > 0, f"para4: N={N}, K={K} (K ate {256 * BLK})")
+        Nt, Kt = -(-N // 16), -(-K // 128)
+        P = (torch.empty(Nt, Kt, 64, 16, dtype=torch.uint8, device=m.device),
+             torch.empty(Nt, Kt, 16, 128 // BLK, dtype=torch.bfloat16, device=m.device), torch.empty(N, dtype=torch.int16, device=m.device))
+        self._lanca("para4", "jt_para4", (m, E, *P, N, K), dict(W=m, WE=E), (N, K))
+        return P
+
+    def _gemv4(self, op, modo, X, P, R=None):
+        self.reg.confere_bloco("X", X)
+        (x, xE), (w, esc, r) = X, P
+        (M, K), N = x.shape, r.numel()
+        Nt, Kt = -(-N // 16), -(-K // 128)
+        if not (w.dtype == torch.uint8 and esc.dtype == torch.bfloat16 and r.dtype == torch.int16 and w.shape == (Nt, Kt, 64, 16)
+                and esc.shape == (Nt, Kt, 16, 128 // BLK) and r.dim() == 1 and w.is_contiguous() and esc.is_contiguous() and r.is_contiguous()
+                and 0 < K <= 256 * BLK and N > 0 and (modo == 1 or N % BLK == 0) and x.get_device() == w.get_device() == esc.get_device() == r.get_device()):
+            self.reg.falha(f"{op}: X {tuple(x.shape)}, pesos {tuple(w.shape)} {w.dtype}, escalas {tuple(esc.shape)} {esc.dtype}, expoentes "
+                           f"{tuple(r.shape)} {r.dtype} (de para4, com BLK={BLK}, K ate {256 * BLK}; N multiplo de {BLK}, ou cru)")
+        ent = dict(X=x, XE=xE, W=w, escalas=esc, R=r)
+        if R is not None:
+            self.reg.confere_bloco("R", R)
+            if R[0].shape != (M, N):
+                self.reg.falha(f"{op}: R com forma {tuple(R[0].shape)}, esperado {(M, N)}")
+            ent.update(res=R[0], resE=R[1])
+        if modo == 1:
+            Y = (torch.empty(M, N, dtype=torch.int32, device=x.device), torch.empty(M, N, dtype=torch.int16, device=x.device))
+        else:
+            Y = self._novo_bloco(M, N, x.device)
+        self._lanca(op, "jt_gemv4", (x, xE, w, esc, r, *(R or (None, None)), *Y, M, N, K, modo), ent, (M, N))
+        return Y
+
+    def gemv4(self, X, P, cru=False):
+        """X [M, K] times the transpose of the 4-bit weights P [N, K] (para4), meant for a few rows (any M works): a block
+        tensor, or a raw one (cru=True, any N). The block format's sum, rounded per block as `gemm` rounds, with a guard
+        of BLK / 16 (jt_gemv4 in include/jatai.h has the formula)."""
+        return self._gemv4("gemv4_cru" if cru else "gemv4", int(cru), X, P)
+
+    def gemv4_soma(self, X, P, R):
+        """soma(R, gemv4(X, P)) in one launch."""
+        return self._gemv4("gemv4_soma", 2, X, P, R)
+
+    def gemv4_relu2(self, X, P):
+        """relu2(gemv4(X, P)) in one launch."""
+        return self._gemv4("gemv4_relu2", 3, X, P)
