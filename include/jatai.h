@@ -192,7 +192,7 @@ int jt_atencao_back_ws_qs(const void* gom, const void* goE, const void* qm, cons
  * [npag][camadas][2: keys, values][Hk][pag][hd], E int8 [npag][camadas][2][Hk][pag][hd / min(hd, BLK)]; hd 4, 16, 32, 64
  * or 128, pag a power of two from 16 to 1024. A token at position j of sequence b is slot j % pag of page tab[b][j / pag].
  * Rows: a block tensor qm int8 [M, (H + 2 Hk) hd], qE; sequence b's newest tokens are the rows ini[b] .. ini[b + 1] - 1
- * (ini null: row b), at positions comp[b] - (ini[b + 1] - ini[b]) .. comp[b] - 1. tab int32 [B][P], comp int32 [B], ini
+ * (ini null: row b, none where comp[b] is 0), at positions comp[b] - (ini[b + 1] - ini[b]) .. comp[b] - 1. tab int32 [B][P], comp int32 [B], ini
  * int32 [B + 1] are device arrays read by the kernels; novos and teto (<= P pag) bound a sequence's rows and comp. A
  * sequence outside those bounds and a page outside 0 .. npag - 1 that a row needs raise E_ARG; neither is read. */
 int jt_cache_grava(const void* qm, const void* qE, void* cm, void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag,

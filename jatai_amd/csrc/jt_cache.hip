@@ -16,15 +16,15 @@ namespace atc {
 struct Seq { int b, i, ok; };                    // sequence of a row, its position, whether it has one
 
 struct Lote {
-    const int *tab, *comp, *ini;                 // [B][P], [B], [B + 1]; ini null: one row per sequence
+    const int *tab, *comp, *ini;                 // [B][P], [B], [B + 1]; ini null: row b is sequence b's
     int B, P, M, lgpag, npag, novos, teto;       // novos: most rows of a sequence; teto: most tokens
 };
 
 // first row, row count and length of sequence b; false (and E_ARG, from the one lane that asks) where they are malformed
 __device__ __forceinline__ bool sequencia(const Lote& L, int b, int& r0, int& n, int& comp, int kid, bool relata) {
-    r0 = L.ini ? L.ini[b] : b;
-    n = (L.ini ? L.ini[b + 1] : b + 1) - r0;
     comp = L.comp[b];
+    r0 = L.ini ? L.ini[b] : b;
+    n = L.ini ? L.ini[b + 1] - r0 : min(comp, 1);                     // without starts, an empty sequence has no row
     const bool ok = r0 >= 0 && n >= 0 && r0 <= L.M - n && n <= L.novos && comp >= n && comp <= L.teto;
     if (!ok && relata) reporta(E_ARG, kid, r0, comp, b);
     return ok;
@@ -47,6 +47,7 @@ __device__ __forceinline__ Seq acha(const Lote& L, int r, int kid, bool relata) 
     if (s.b < 0) return s;
     int r0, n, comp;
     s.ok = sequencia(L, s.b, r0, n, comp, kid, relata);
+    s.ok = s.ok && r - r0 < n;
     s.i = comp - n + (r - r0);
     return s;
 }
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(256) k_cache_grava(const int8_t* __restrict__ 
         if (b >= L.B || r < L.ini[b]) return;                                           // behind the last sequence
     } else if ((b = r) >= L.B) return;
     int r0, n, comp;
-    if (!atc::sequencia(L, b, r0, n, comp, kid, kvh == 0 && c == 0)) return;
+    if (!atc::sequencia(L, b, r0, n, comp, kid, kvh == 0 && c == 0) || r - r0 >= n) return;
     const int j = comp - n + (r - r0), pag = 1 << L.lgpag;
     const int p = L.tab[(long long)b * L.P + (j >> L.lgpag)];
     if ((unsigned)p >= (unsigned)L.npag) {

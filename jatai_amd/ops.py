@@ -69,7 +69,7 @@ def carrega_lib(caminho=LIB):
 class Lote(typing.NamedTuple):
     """The sequences of one generation call. tabela int32 [B, P]: the cache page of each run of slots (-1: none); comp
     int32 [B]: tokens of each sequence, the new ones among them; ini int32 [B + 1]: first row of each sequence's new
-    tokens, and the end of the last's (None: row b is sequence b's one new token). novos and teto bound, on the host,
+    tokens, and the end of the last's (None: row b is sequence b's one new token, if comp[b] > 0). novos and teto bound, on the host,
     the new tokens of a sequence and comp; the tensors are read when the kernels run, so a captured graph follows them."""
     tabela: torch.Tensor
     comp: torch.Tensor
@@ -729,6 +729,8 @@ class OpsHip:
         for n, t, f in (("tabela", tab, (B, tab.shape[-1])), ("comp", comp, (B,))) + ((("ini", ini, (B + 1,)),) if ini is not None else ()):
             if not (t.dtype == torch.int32 and t.is_contiguous() and t.shape == f and t.is_cuda and t.get_device() == m.get_device() and t.numel()):
                 self.reg.falha(f"{op}: {n} {tuple(t.shape)} {t.dtype}, esperado int32 {f} contiguo na GPU de qkv")
+        if ini is None and B > m.shape[0]:
+            self.reg.falha(f"{op}: {B} sequencias para {m.shape[0]} linhas")
         if not (0 <= lote.novos <= 2**30 and 0 <= lote.teto <= min(2**30, tab.shape[1] * pag)):
             self.reg.falha(f"{op}: novos={lote.novos}, teto={lote.teto} para {tab.shape[1]} paginas de {pag}")
         return paginas, camadas, Hk, hd, pag, H, B, tab.shape[1]
