@@ -203,8 +203,8 @@ int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, in
 /* out [M, H hd]: softmax_j(q . k_j / sqrt(hd) - incl[h] (i - j)) . v_j over the visible tokens j <= i of the row's sequence:
  * all (janela 0), or the last janela and the first sumid. Query head h reads head h / (H / Hk); incl float [H] or null.
  * tipo 0: block tensor (out int8, outE), 1: bfloat16, 2: fp32. Rows of no sequence come out as zeros. ws: workspace of
- * jt_atencao_cache_ws_bytes bytes, 16-byte aligned, not shared by calls that overlap. */
-long long jt_atencao_cache_ws_bytes(int M, int H, int hd, int teto, int janela, int sumid);
+ * jt_atencao_cache_ws_bytes bytes (0: none, ws may be null; it depends on the block size), 16-byte aligned, not shared by calls that overlap. */
+long long jt_atencao_cache_ws_bytes(int M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo);
 int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag,
                      const void* tab, const void* comp, const void* ini, const void* incl, void* out, void* outE, int M, int B, int P,
                      int novos, int teto, int H, int janela, int sumid, int tipo, void* ws, long long ws_bytes, int kid);

@@ -1045,20 +1045,36 @@ int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, in
     return 0;
 }
 
-// Splits of a row's visible tokens, and tokens per split: as many as fill the chip (8 workgroups of 4 waves per CU), each with
-// at least one step of a workgroup's loop (256 tokens at head width 64).
-static void atc_divide(long long M, int H, int hd, int teto, int janela, int sumid, int& S, int& fatia) {
-    const long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto);
-    const long long passo = hd <= 16 ? 1024 : 16384 / hd, max_s = (nv + passo - 1) / passo;
-    const long long s = std::min(std::max(2048 / std::max(M * H, 1LL), 1LL), max_s);
-    fatia = (int)(((nv + s - 1) / s + passo - 1) / passo * passo);
-    S = (int)((nv + fatia - 1) / fatia);
+// How a call runs. mf: several rows share keys and values (k_atc_mf, 64 rows a workgroup, por_seq workgroups a sequence);
+// else a row each (k_atc_um). S splits of the visible tokens, `fatia` tokens (mf: 64-token tiles) each: as many as fill
+// the chip, each with at least one step (um) or 4 tiles (mf) of a workgroup's loop. direto: one split, and every block
+// of the output lies in a head, so the kernel writes it and there is no join.
+struct PlanoAtc { bool mf, direto; int por_seq, S, fatia; };
+static PlanoAtc atc_plano(long long M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo) {
+    PlanoAtc p;
+    const long long linhas = (long long)novos * (H / Hk);            // that share a kv head's keys, at most
+    p.mf = linhas > 1;
+    p.por_seq = (int)std::max(1LL, (linhas + 63) / 64);
+    long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto), passo, wgs;
+    if (p.mf) {                                                      // in tiles: a window's may begin and end inside one, the first tokens' too
+        const long long nt = (teto + 63LL) / 64;
+        nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, 64LL) + 62) / 64 + 1 + (sumid + 63LL) / 64) : nt);
+        passo = 4;
+        wgs = (long long)B * p.por_seq * Hk;
+    } else {
+        passo = hd <= 16 ? 1024 : 16384 / hd;
+        wgs = M * H;
+    }
+    const long long s = std::min(std::max((p.mf ? 1024 : 2048) / std::max(wgs, 1LL), 1LL), (nv + passo - 1) / passo);
+    p.fatia = (int)(((nv + s - 1) / s + passo - 1) / passo * passo);
+    p.S = (int)((nv + p.fatia - 1) / p.fatia);
+    p.direto = p.mf && p.S == 1 && (tipo != 0 || hd >= g_blk);
+    return p;
 }
-long long jt_atencao_cache_ws_bytes(int M, int H, int hd, int teto, int janela, int sumid) {
-    if (M <= 0 || H <= 0 || hd <= 0 || teto < 0 || teto > (1 << 30)) return 0;
-    int S, fatia;
-    atc_divide(M, H, hd, teto, janela, sumid, S, fatia);
-    return (long long)M * H * S * (hd + 2) * 4 + 16;
+long long jt_atencao_cache_ws_bytes(int M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo) {
+    if (M <= 0 || B <= 0 || H <= 0 || Hk <= 0 || hd <= 0 || novos < 0 || teto < 0 || teto > (1 << 30) || janela < 0 || sumid < 0) return 0;
+    const PlanoAtc p = atc_plano(M, B, H, Hk, hd, novos, teto, janela, sumid, tipo);
+    return p.direto ? 0 : (long long)M * H * p.S * (hd + 2) * 4 + 16;
 }
 int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag,
                      const void* tab, const void* comp, const void* ini, const void* incl, void* out, void* outE, int M, int B, int P,
@@ -1067,23 +1083,24 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
     if (M == 0) return 0;
     if (!qm || !qE || !out || !alinhados(qm, out, ws) || H <= 0 || H > 65535 || H % Hk || (long long)(H + 2LL * Hk) * hd % g_blk) return (int)hipErrorInvalidValue;
     if (janela < 0 || sumid < 0 || tipo < 0 || tipo > 2 || (tipo == 0 && (!outE || H * hd % g_blk))) return (int)hipErrorInvalidValue;
-    if (!ws || ws_bytes < jt_atencao_cache_ws_bytes(M, H, hd, teto, janela, sumid)) return (int)hipErrorInvalidValue;
-    int S, fatia;
-    atc_divide(M, H, hd, teto, janela, sumid, S, fatia);
-    const long long camada_m = 2LL * Hk * pag * hd, camada_e = 2LL * Hk * pag * grupos(hd), partes = (long long)M * H * S;
-    float *ml = (float*)ws, *po = ml + (2 * partes + 3) / 4 * 4;
+    const PlanoAtc p = atc_plano(M, B, H, Hk, hd, novos, teto, janela, sumid, tipo);
+    if (!p.direto && (!ws || ws_bytes < jt_atencao_cache_ws_bytes(M, B, H, Hk, hd, novos, teto, janela, sumid, tipo))) return (int)hipErrorInvalidValue;
+    if (p.S > 65535 || (long long)(B + 1) * p.por_seq > 0x7fffffff) return (int)hipErrorInvalidValue;
+    const long long camada_m = 2LL * Hk * pag * hd, camada_e = 2LL * Hk * pag * grupos(hd), partes = (long long)M * H * p.S;
+    float *ml = p.direto ? nullptr : (float*)ws, *po = p.direto ? nullptr : ml + (2 * partes + 3) / 4 * 4;
     const atc::Args a{(const int8_t*)qm, (const int8_t*)qE, (const int8_t*)cm + camada * camada_m, (const int8_t*)cE + camada * camada_e,
-                      (const float*)incl, ml, po, camadas * camada_m, camadas * camada_e,
+                      (const float*)incl, ml, po, out, (int8_t*)outE, camadas * camada_m, camadas * camada_e,
                       atc::Lote{(const int*)tab, (const int*)comp, (const int*)ini, B, P, M, ilog2(pag), npag, novos, teto},
-                      H, Hk, ilog2(g_blk), janela, sumid, S, fatia, kid};
-#define F(HD, GS) (k_atc_um<HD, GS><<<dim3(M, H, S), 256, 0, g_stream>>>(a))
+                      H, Hk, ilog2(g_blk), janela, sumid, p.S, p.fatia, tipo, kid};
+#define F(HD, GS) (p.mf ? k_atc_mf<HD, GS><<<dim3((B + 1) * p.por_seq, Hk, p.S), 256, 0, g_stream>>>(a, p.por_seq) \
+                        : k_atc_um<HD, GS><<<dim3(M, H, p.S), 256, 0, g_stream>>>(a))
     POR_CABECA(F)
 #undef F
     int rc = fim();
-    if (rc) return rc;
+    if (rc || p.direto) return rc;
     const int C = H * hd;
     const dim3 grade(M, (C + 1023) / 1024);
-#define J(BL, T) (k_atc_junta<BL, T><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, S, kid))
+#define J(BL, T) (k_atc_junta<BL, T><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid))
     if (tipo == 1) J(32, 1);
     else if (tipo == 2) J(32, 2);
     else if (g_blk == 32) J(32, 0);

@@ -110,11 +110,26 @@ namespace atc {
 struct Args {
     const int8_t *qm, *qE, *cm, *cE;             // cm, cE: at the layer
     const float* incl;                           // null: no bias
-    float *ml, *o;                               // partial results: (maximum, sum) and outputs per (row, head, split)
+    float *ml, *o;                               // partial results: (maximum, sum) and outputs per (row, head, split); null:
+    void* out;                                   // none, the kernel itself writes out (outE) as `tipo` (k_atc_junta's) says
+    int8_t* outE;
     long long pag_m, pag_e;
     Lote L;
-    int H, Hk, lgblk, janela, sumid, S, fatia, kid;   // S splits of `fatia` visible tokens each
+    int H, Hk, lgblk, janela, sumid, S, fatia, tipo, kid;   // S splits of `fatia` visible tokens (k_atc_mf: 64-token tiles) each
 };
+
+// Scores stay in nats (a factor of log2 e would round each of them once more) and become powers of two as
+// exp2(s log2 e - m log2 e), one FMA whose rounding is small where the weight is large. The rounding of m log2 e is common to
+// all weights under a maximum, and the factor between two maxima takes the same rounded products (never contracted into an FMA), so that
+// it fits them, and is exactly 1 where the maximum stays.
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float vezes_log2e(float m) {
+#pragma clang fp contract(off)
+    return m * LOG2E;
+}
+__device__ __forceinline__ float peso(float s, float mL) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, LOG2E, -mL)); }
+// 2^(m log2 e - M log2 e) for m <= M, 0 where m is -inf (also M)
+__device__ __forceinline__ float fator(float m, float M) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(vezes_log2e(m) - vezes_log2e(M)); }
 
 template <int LPK>
 __device__ __forceinline__ float soma_grupo(float v) {               // over LPK consecutive lanes, to all of them
@@ -130,7 +145,7 @@ __device__ __forceinline__ float soma_grupo(float v) {               // over LPK
 
 // One row (token, query head) and one split of its visible tokens per workgroup. Softmax in one pass: every group of LPK
 // lanes (a key's head row, 16 bytes a lane) keeps the running maximum m, sum l and output o of the keys it has seen,
-//   u = 2^(Eq + Ek) (mq . mk) / sqrt(hd) - incl (i - j), in units of log2 e;  p = 2^(u - m);  o += p 2^Ev mv,
+//   u = 2^(Eq + Ek) (mq . mk) / sqrt(hd) - incl (i - j);  p = exp(u - m);  o += p 2^Ev mv,
 // and they are joined at the end (lanes, waves, then the splits by k_atc_junta). Products of mantissas are exact in int32
 // (v_dot4), statistics and outputs fp32. The visible tokens are numbered x = 0 .. nvis - 1 without gaps, the first tokens
 // then the window, so no masked key is read.
@@ -153,8 +168,7 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
 #pragma unroll
     for (int k = 0; k < VB / 4; k++) qv[k] = reinterpret_cast<const int*>(a.qm + (long long)r * ld + col)[k];
     const int eq = a.qE[(long long)r * (ld >> a.lgblk) + (col >> a.lgblk)];
-    constexpr float LOG2E = 1.4426950408889634f;
-    const float esc = LOG2E / __builtin_sqrtf((float)HD), incl = a.incl ? a.incl[h] * LOG2E : 0.f;
+    const float esc = 1.f / __builtin_sqrtf((float)HD), incl = a.incl ? a.incl[h] : 0.f;
 
     float m = -INFINITY, l = 0.f, o[VB];
 #pragma unroll
@@ -198,14 +212,14 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
             t[u] = vis[u] ? t[u] : -INFINITY;
             mn = fmaxf(mn, t[u]);
         }
-        const float ref = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - ref);
+        const float mL = mn == -INFINITY ? 0.f : atc::vezes_log2e(mn), al = atc::fator(m, mn);
         m = mn;
         l *= al;
 #pragma unroll
         for (int d = 0; d < VB; d++) o[d] *= al;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const float e = __builtin_amdgcn_exp2f(t[u] - ref);
+            const float e = atc::peso(t[u], mL);
             l += e;
             const float pv = vis[u] ? __builtin_ldexpf(e, ev[u]) : 0.f;
 #pragma unroll
@@ -217,7 +231,7 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
     float M = m;
 #pragma unroll
     for (int x = LPK; x < 64; x *= 2) M = fmaxf(M, __shfl_xor(M, x));
-    const float es = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    const float es = atc::fator(m, M);
     l *= es;
 #pragma unroll
     for (int x = LPK; x < 64; x *= 2) l += __shfl_xor(l, x);
@@ -250,7 +264,7 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
     for (int k = 1; k < NW; k++) MM = fmaxf(MM, sm[k]);
 #pragma unroll
     for (int k = 0; k < NW; k++) {
-        const float f = sm[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[k] - MM);
+        const float f = atc::fator(sm[k], MM);
         LL += sl[k] * f;
         oo += so[k][threadIdx.x] * f;
     }
@@ -259,26 +273,30 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
     if (threadIdx.x == 0) { a.ml[2 * part] = MM; a.ml[2 * part + 1] = LL; }
 }
 
-// fp32 values of a block (LPB lanes x NV) to int8 mantissas and an exponent, rounded once, half to even: E = binary
-// exponent of the largest |v| - 7, one up where a mantissa passes 127; the products by 2^-E are exact. A block below
+// Exponent of a block of fp32 values in the int8 format, from the bits of the largest |v|, and the scale 2^-E: E = binary
+// exponent - 7, one up where the largest mantissa rounds past 127 (half to even; products by 2^-E are exact). A block below
 // 2^-126 is zero; one that holds an infinity or a NaN raises E_EXP and is zero.
+__device__ __forceinline__ int expoente_f32(int bits, float& f, int kid, long long idx) {
+    int E = (bits >> 23) - 133;
+    f = __builtin_ldexpf(1.f, -E);
+    if (__builtin_rintf(__int_as_float(bits) * f) > 127.f) { E++; f *= 0.5f; }
+    if (bits >= 0x7f800000) reporta(E_EXP, kid, idx, E, bits);
+    return E < -126 || bits >= 0x7f800000 ? E_ZERO : E;
+}
+// a block of LPB lanes x NV values to int8 mantissas; returns its exponent
 template <int NV, int LPB>
 __device__ __forceinline__ int quant_f32(const float (&v)[NV], int8_t (&q)[NV], int kid, long long idx0) {
     int bits = 0;
 #pragma unroll
     for (int k = 0; k < NV; k++) bits = max(bits, __float_as_int(v[k]) & 0x7fffffff);
-    bits = g_max<LPB>(bits);
-    int E = (bits >> 23) - 133;
-    float f = __builtin_ldexpf(1.f, -E);
-    if (__builtin_rintf(__int_as_float(bits) * f) > 127.f) { E++; f *= 0.5f; }
-    if (bits >= 0x7f800000) reporta(E_EXP, kid, idx0, E, bits);
-    const bool zero = E < -126 || bits >= 0x7f800000;
+    float f;
+    const int E = expoente_f32(g_max<LPB>(bits), f, kid, idx0);
 #pragma unroll
-    for (int k = 0; k < NV; k++) q[k] = zero ? 0 : (int8_t)(int)__builtin_rintf(v[k] * f);
-    return zero ? E_ZERO : E;
+    for (int k = 0; k < NV; k++) q[k] = E == E_ZERO ? 0 : (int8_t)(int)__builtin_rintf(v[k] * f);
+    return E;
 }
 
-// Joins the splits of a row and head, o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s (zeros for a row without visible
+// Joins the splits of a row and head, o = sum exp(m_s - m) o_s / sum exp(m_s - m) l_s (zeros for a row without visible
 // tokens), 4 columns a thread, and writes the row as a block tensor (TIPO 0), bfloat16 (1) or fp32 (2).
 template <int BLK, int TIPO>
 __global__ void __launch_bounds__(256) k_atc_junta(const float* __restrict__ ml, const float* __restrict__ po, void* __restrict__ out,
@@ -291,7 +309,7 @@ __global__ void __launch_bounds__(256) k_atc_junta(const float* __restrict__ ml,
     for (int s = 0; s < S; s++) {
         const float m = ml[2 * (part + s)];
         if (m == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(m - M);
+        const float f = atc::fator(m, M);
         L += f * ml[2 * (part + s) + 1];
         const float4 x = *reinterpret_cast<const float4*>(po + (part + s) * hd + col % hd);
         v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
@@ -312,6 +330,290 @@ __global__ void __launch_bounds__(256) k_atc_junta(const float* __restrict__ ml,
         *reinterpret_cast<float4*>((float*)out + x) = make_float4(v[0], v[1], v[2], v[3]);
     }
 }
+
+// Several rows that share keys and values (new tokens of a sequence, query heads of a group): 64 of them per workgroup, 16 a
+// wave, on matrix cores; the workgroup walks its keys in tiles of 64. Row rho of a (sequence, kv head) is token rho / Gq,
+// head rho % Gq of the group.
+//   S^T = K Q^T by i8 MFMA, exact in int32, one accumulator per exponent group: a lane holds one row (lane % 16) and 4 keys of
+//   each 16, so maxima and sums are in-lane but for two exchanges, and P^T is the next product's operand as it stands.
+//   O^T = V^T P^T by bf16 MFMA: V's values m 2^E are exact in bf16 (8 bits), P is three bf16 pieces, exact too (one piece
+//   would leave 2^-8 of every weight, two 2^-16). V^T comes from row-major LDS by transposing reads.
+// Keys and values are staged once per workgroup, two tiles in LDS: the next tile's loads are in flight while this one is
+// computed, its page numbers one tile earlier still. Slots no row sees are staged as zeros, whatever they hold. The running maximum is
+// raised (and O rescaled) only where a tile exceeds it by 5 nats: weights are then at most e^5, which costs fp32 no precision.
+template <int HD, int GS>
+__global__ void __launch_bounds__(256) k_atc_mf(atc::Args a, int por_seq) {
+    typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+    typedef short s4_t __attribute__((ext_vector_type(4)));
+    typedef float f4_t __attribute__((ext_vector_type(4)));
+    typedef int i4_t __attribute__((ext_vector_type(4)));
+    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 64;
+    constexpr int NM = HD < 32 ? 1 : HD / 32, MPG = NM / G, DT = HD < 16 ? 1 : HD / 16;       // MFMAs of a score, per group; tiles of O
+    constexpr int KS = HD < 16 ? 4 : HD + 8, VS = 16 * DT + 8;                                // LDS rows, in values
+    constexpr int NT = 2 * TK * LPK, IT = (NT + 255) / 256, NK = IT == 4 ? 2 : 1;             // staging: tasks, per thread; keys of a thread
+    __shared__ __align__(16) int8_t sk[2][TK * KS];
+    __shared__ __align__(16) __bf16 sv[2][TK * VS];
+    __shared__ __align__(16) float sf[2][G * TK];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk, C = a.H * HD;
+    const int b = blockIdx.x / por_seq, tile = por_seq - 1 - blockIdx.x % por_seq;            // a sequence's last rows, the longest, first
+
+    // a row without visible tokens: its outputs (or the marks of its splits) for this workgroup's heads
+    auto vazia = [&](long long r) {
+        for (int x = threadIdx.x; x < Gq * HD; x += 256) {
+            const int h = hk * Gq + x / HD;
+            const long long o = r * C + h * HD + x % HD;
+            if (a.ml) {
+                if (x % HD == 0) { float* y = a.ml + 2 * ((r * a.H + h) * a.S + blockIdx.z); y[0] = -INFINITY; y[1] = 0.f; }
+            } else if (a.tipo == 0) {
+                reinterpret_cast<int8_t*>(a.out)[o] = 0;
+                if (!((h * HD + x % HD) & ((1 << a.lgblk) - 1))) a.outE[o >> a.lgblk] = E_ZERO;
+            } else if (a.tipo == 1) reinterpret_cast<__bf16*>(a.out)[o] = (__bf16)0.f;
+            else reinterpret_cast<float*>(a.out)[o] = 0.f;
+        }
+    };
+    if (b == a.L.B) {                                                 // rows of no sequence
+        const int ini = a.L.ini ? a.L.ini[0] : 0, fim = a.L.ini ? a.L.ini[a.L.B] : a.L.B;
+        for (long long x = tile; x < min(ini, a.L.M); x += por_seq) vazia(x);
+        for (long long x = max(fim, 0) + (long long)tile; x < a.L.M; x += por_seq) vazia(x);
+        return;
+    }
+    int r0, n, comp;
+    if (!atc::sequencia(a.L, b, r0, n, comp, a.kid, threadIdx.x == 0 && hk == 0 && blockIdx.z == 0 && tile == 0)) {
+        const long long fim = a.L.ini ? (long long)a.L.ini[b + 1] : b + 1;
+        if (tile == 0)
+            for (long long r = max(r0, 0); r < min(fim, (long long)a.L.M); r++) vazia(r);
+        return;
+    }
+    if (!a.L.ini && n == 0 && tile == 0 && r0 < a.L.M) vazia(r0);
+    const int linhas = n * Gq, rho0 = tile * 64;
+    if (rho0 >= linhas) return;
+    const int i_lo = comp - n + rho0 / Gq, i_hi = comp - n + min(rho0 + 63, linhas - 1) / Gq;
+    const int lo = a.janela > 0 ? max(0, i_lo + 1 - a.janela) : 0, ns = min(a.sumid, lo), nst = (ns + TK - 1) / TK, prim = max(nst, lo / TK);
+    const int T = nst + i_hi / TK - prim + 1, t0 = min((long long)blockIdx.z * a.fatia, (long long)T), t1 = min(t0 + a.fatia, T);
+
+    // this lane's row
+    const int rho = rho0 + 16 * w + lr, rc = min(rho, linhas - 1), h = hk * Gq + rc % Gq, i = comp - n + rc / Gq;
+    const int w_hi = comp - n + min(rho0 + 16 * w + 15, linhas - 1) / Gq;                     // the wave's last position
+    const bool tem = rho0 + 16 * w < linhas;
+    const long long r = r0 + rc / Gq;
+    const int ld = (a.H + 2 * a.Hk) * HD;
+    const float incl = a.incl ? a.incl[h] : 0.f;
+    long q[NM];
+    float fq[G];
+#pragma unroll
+    for (int k = 0; k < NM; k++) {
+        const int8_t* p = a.qm + r * ld + h * HD + 32 * k + 8 * c;
+        if constexpr (HD >= 32) q[k] = *reinterpret_cast<const long*>(p);
+        else if constexpr (HD == 16) q[k] = c < 2 ? *reinterpret_cast<const long*>(p) : 0;
+        else q[k] = c == 0 ? (long)*reinterpret_cast<const unsigned*>(p) : 0;
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++)
+        fq[g] = __builtin_ldexpf(1.f / __builtin_sqrtf((float)HD), a.qE[r * (ld >> a.lgblk) + ((h * HD + g * GS) >> a.lgblk)]);
+
+    const int pag = 1 << a.L.lgpag;
+    auto j0_de = [&](int t) { return TK * (t < nst ? t : t - nst + prim); };
+    constexpr int OCULTA = -2;                                        // a key that no row of the workgroup sees
+    int pg[NK];
+    int4 dm[IT];
+    int de[IT];
+    auto chave = [&](int k) { return (int)((threadIdx.x / LPK + 32 * k) % TK); };
+    auto le_paginas = [&](int t) {
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            const int j = j0_de(t) + chave(k);
+            const bool vis = t < t1 && j <= i_hi && (j >= lo || j < ns);
+            const int p = a.L.tab[(long long)b * a.L.P + (vis ? j >> a.L.lgpag : 0)];
+            pg[k] = vis ? p : OCULTA;
+            if (vis && (unsigned)p >= (unsigned)a.L.npag) {
+                if (hk == 0 && threadIdx.x % LPK == 0) reporta(E_ARG, a.kid, (long long)b * a.L.P + (j >> a.L.lgpag), p, j);
+                pg[k] = OCULTA;
+            }
+        }
+    };
+    // task: a chunk of VB bytes of a key (first TK LPK tasks) or a value, and its exponent
+    auto le_dados = [&](int t) {
+#pragma unroll
+        for (int x = 0; x < IT; x++) {
+            const int tarefa = threadIdx.x + 256 * x, k = NK == 2 ? x & 1 : 0, kv = tarefa / (TK * LPK), cc = tarefa % LPK;
+            dm[x] = make_int4(0, 0, 0, 0);
+            de[x] = -127;
+            if (tarefa < NT && pg[k] != OCULTA) {
+                const long long vaga = ((long long)kv * a.Hk + hk) * pag + ((j0_de(t) + chave(k)) & (pag - 1));
+                const int8_t* p = a.cm + pg[k] * a.pag_m + vaga * HD + cc * VB;
+                if constexpr (VB == 16) dm[x] = *reinterpret_cast<const int4*>(p);
+                else dm[x].x = *reinterpret_cast<const int*>(p);
+                de[x] = a.cE[pg[k] * a.pag_e + vaga * G + cc * VB / GS];
+            }
+        }
+    };
+    auto guarda = [&](int buf) {
+#pragma unroll
+        for (int x = 0; x < IT; x++) {
+            const int tarefa = threadIdx.x + 256 * x, k = NK == 2 ? x & 1 : 0, kv = tarefa / (TK * LPK), cc = tarefa % LPK, key = chave(k);
+            if (tarefa >= NT) continue;
+            const float e = __builtin_ldexpf(1.f, de[x]);
+            if (kv == 0) {
+                int8_t* p = &sk[buf][key * KS + cc * VB];
+                if constexpr (VB == 16) {
+                    reinterpret_cast<int2*>(p)[0] = make_int2(dm[x].x, dm[x].y);
+                    reinterpret_cast<int2*>(p)[1] = make_int2(dm[x].z, dm[x].w);
+                } else *reinterpret_cast<int*>(p) = dm[x].x;
+                if (cc * VB % GS == 0) sf[buf][cc * VB / GS * TK + key] = e;
+            } else {
+                const int y[4] = {dm[x].x, dm[x].y, dm[x].z, dm[x].w};
+                __bf16* p = &sv[buf][key * VS + cc * VB];
+#pragma unroll
+                for (int d = 0; d < VB; d += 8) {
+                    b8_t z;
+#pragma unroll
+                    for (int k8 = 0; k8 < 8; k8++) z[k8] = (__bf16)(d + k8 < VB ? e * (float)(int8_t)(y[(d + k8) / 4 % 4] >> (8 * (k8 % 4))) : 0.f);
+                    *reinterpret_cast<b8_t*>(p + d) = z;
+                }
+                if constexpr (HD < 16) *reinterpret_cast<b8_t*>(p + 8) = b8_t{};
+            }
+        }
+    };
+
+    float m = -INFINITY, l = 0.f;
+    f4_t o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = f4_t{0, 0, 0, 0};
+    if (t0 < t1) {
+        le_paginas(t0);
+        le_dados(t0);
+        le_paginas(t0 + 1);
+        guarda(0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; t++) {
+        const int buf = (t - t0) & 1, j0 = j0_de(t);
+        if (t + 1 < t1) { le_dados(t + 1); le_paginas(t + 2); }
+        if (tem && j0 <= w_hi) {
+            float s[16];
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    i4_t p = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = g * MPG; k < (g + 1) * MPG; k++) {
+                        const int8_t* y = &sk[buf][(16 * kt + lr) * KS + 32 * k + 8 * c];
+                        long kf;
+                        if constexpr (HD >= 32) kf = *reinterpret_cast<const long*>(y);
+                        else if constexpr (HD == 16) kf = c < 2 ? *reinterpret_cast<const long*>(y) : 0;
+                        else kf = c == 0 ? (long)*reinterpret_cast<const unsigned*>(y) : 0;
+                        p = __builtin_amdgcn_mfma_i32_16x16x32_i8(kf, q[k], p, 0, 0, 0);
+                    }
+                    const float4 f = *reinterpret_cast<const float4*>(&sf[buf][g * TK + 16 * kt + 4 * c]);
+                    x[0] += (float)p[0] * f.x * fq[g]; x[1] += (float)p[1] * f.y * fq[g];
+                    x[2] += (float)p[2] * f.z * fq[g]; x[3] += (float)p[3] * f.w * fq[g];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) s[4 * kt + k] = x[k] - incl * (float)(i - j0 - 16 * kt - 4 * c - k);
+            }
+            // every key of the tile visible to every row of the workgroup: nothing to mask
+            if (j0 + TK - 1 > i_lo || (a.janela > 0 && j0 <= i_hi - a.janela && j0 + TK > a.sumid)) {
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const int j = j0 + 16 * (k / 4) + 4 * c + k % 4;
+                    const bool vis = j <= i && (a.janela <= 0 || j > i - a.janela || j < a.sumid);
+                    s[k] = vis ? s[k] : -INFINITY;
+                }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int k = 1; k < 16; k++) mx = fmaxf(mx, s[k]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (__any(mx > m + 5.f)) {
+                const float mn = fmaxf(m, mx), al = atc::fator(m, mn);
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] *= al;
+            }
+            const float mL = m == -INFINITY ? 0.f : atc::vezes_log2e(m);
+            i4_t p[3][2];                                             // a weight's 24 bits in three bf16 pieces, exactly
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+                int y[3][2];
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const float e = atc::peso(s[k + x], mL);
+                    l += e;
+                    y[0][x] = __float_as_int(e);
+                    const float e1 = e - __int_as_float(y[0][x] & 0xffff0000);
+                    y[1][x] = __float_as_int(e1);
+                    y[2][x] = __float_as_int(e1 - __int_as_float(y[1][x] & 0xffff0000));
+                }
+#pragma unroll
+                for (int x = 0; x < 3; x++) p[x][k / 8][k % 8 / 2] = (int)__builtin_amdgcn_perm((unsigned)y[x][1], (unsigned)y[x][0], 0x07060302u);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    // lane 16 c + x reads row 4 c + x / 4, columns 4 (x % 4) ..; it receives column x of the 4 rows
+                    const __bf16* y = &sv[buf][(32 * kk + 4 * c + lr / 4) * VS + 16 * d + 4 * (lr % 4)];
+                    typedef __attribute__((address_space(3))) s4_t* lds4;
+                    const s4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(y)), v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(y + 16 * VS));
+                    const b8_t v = __builtin_bit_cast(b8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int x = 0; x < 3; x++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(b8_t, p[x][kk]), o[d], 0, 0, 0);
+                }
+        }
+        if (t + 1 < t1) guarda(buf ^ 1);
+        __syncthreads();
+    }
+    if (rho >= linhas) return;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (a.ml) {
+        const long long part = (r * a.H + h) * a.S + blockIdx.z;
+        if (c == 0) { a.ml[2 * part] = m; a.ml[2 * part + 1] = l; }
+        if (HD >= 16 || c == 0)
+#pragma unroll
+            for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(a.o + part * HD + 16 * d + 4 * c) = o[d];
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] *= inv;
+    const long long x = r * C + h * HD;
+    if (a.tipo == 0) {                                                // one block of the head's: GS = BLK here
+        if constexpr (HD >= 32) {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                constexpr int DG = DT / G;
+                int bits = 0;
+#pragma unroll
+                for (int d = 0; d < 4 * DG; d++) bits = max(bits, __float_as_int(o[g * DG + d / 4][d % 4]) & 0x7fffffff);
+                bits = max(bits, __shfl_xor(bits, 16));
+                bits = max(bits, __shfl_xor(bits, 32));
+                float f;
+                const int E = expoente_f32(bits, f, a.kid, x + g * GS);
+#pragma unroll
+                for (int d = g * DG; d < (g + 1) * DG; d++) {
+                    int8_t z[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) z[k] = E == E_ZERO ? 0 : (int8_t)(int)__builtin_rintf(o[d][k] * f);
+                    grava_i8<4, false>((int8_t*)a.out + x + 16 * d + 4 * c, z);
+                }
+                if (c == 0) a.outE[(x >> a.lgblk) + g] = (int8_t)E;
+            }
+        }
+    } else if (HD >= 16 || c == 0) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            typedef __bf16 b4_t __attribute__((ext_vector_type(4)));
+            if (a.tipo == 1) *reinterpret_cast<b4_t*>((__bf16*)a.out + x + 16 * d + 4 * c) = b4_t{(__bf16)o[d][0], (__bf16)o[d][1], (__bf16)o[d][2], (__bf16)o[d][3]};
+            else *reinterpret_cast<f4_t*>((float*)a.out + x + 16 * d + 4 * c) = o[d];
+        }
+    }
+}
+
 
 // ---------------------------------------------------------------------------------------------- values
 // A block or raw tensor as floats (the inverse of de_f32), each value rounded once: block values are exact in both types

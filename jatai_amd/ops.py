@@ -113,15 +113,18 @@ class OpsHip:
     # message that a well-formed launch does not need. A 512^3 product 18.0 -> 14.2 us; the forward of 12 layers op by op
     # 1653 -> 1325 us (an object per int argument, and guards that format their message also when they hold, before).
     def _lanca(self, op, fn, args, entradas, forma, longos=()):
-        if self._blk != BLK:
-            self.reg.exige(self.lib.jt_bloco(BLK) == 0, f"BLK={BLK} not supported (32 or 128)")
-            self._blk = BLK
+        self._bloco_da_lib()
         kid = self.reg.registra(op, entradas, forma)
         conv = list(map(self._a, args))
         for i in longos:
             conv[i] = ctypes.c_longlong(args[i])
         r = getattr(self.lib, fn)(*conv, kid)
         self.reg.depois(kid, r)
+
+    def _bloco_da_lib(self):
+        if self._blk != BLK:
+            self.reg.exige(self.lib.jt_bloco(BLK) == 0, f"BLK={BLK} not supported (32 or 128)")
+            self._blk = BLK
 
     def _novo_bloco(self, R, C, dev):
         return torch.empty(R, C, dtype=torch.int8, device=dev), torch.empty(R, C // BLK, dtype=torch.int8, device=dev)
@@ -772,11 +775,13 @@ class OpsHip:
         if not (saida in (None, torch.bfloat16, torch.float32) and 0 <= janela <= 2**30 and 0 <= sumidouros <= 2**30 and (saida is not None or D % BLK == 0)):
             self.reg.falha(f"atencao_cache: janela={janela}, sumidouros={sumidouros}, saida={saida} (None com H hd multiplo de {BLK}, bfloat16 ou float32)")
         Y = self._novo_bloco(M, D, m.device) if saida is None else (torch.empty(M, D, dtype=saida, device=m.device), None)
-        nws = self.lib.jt_atencao_cache_ws_bytes(M, H, hd, lote.teto, janela, sumidouros)
-        ws = torch.empty(nws, dtype=torch.uint8, device=m.device)
+        tipo = {None: 0, torch.bfloat16: 1, torch.float32: 2}[saida]
+        self._bloco_da_lib()
+        nws = self.lib.jt_atencao_cache_ws_bytes(M, B, H, Hk, hd, lote.novos, lote.teto, janela, sumidouros, tipo)
+        ws = torch.empty(nws, dtype=torch.uint8, device=m.device) if nws else None
         self._lanca("atencao_cache", "jt_atencao_cache",
                     (m, E, *C, paginas, camadas, camada, Hk, hd, pag, lote.tabela, lote.comp, lote.ini, incl, *Y, M, B, P, lote.novos, lote.teto, H,
-                     janela, sumidouros, {None: 0, torch.bfloat16: 1, torch.float32: 2}[saida], ws, nws),
+                     janela, sumidouros, tipo, ws, nws),
                     dict(qkv=m, qkvE=E, tabela=lote.tabela, comp=lote.comp), (M, D), longos=(26,))
         return Y if saida is None else Y[0]
 

@@ -133,14 +133,14 @@ def test_guardas_c_sem_gpu():
     grava = dict(qm=p, qE=p, cm=p, cE=p, npag=10, camadas=2, camada=1, Hk=2, hd=64, pag=16, **lote, H=2, kid=0)
     assert lib.jt_cache_grava(*{**grava, "M": 0}.values()) == 0
     ruins = (dict(qm=n), dict(qE=n), dict(cm=n), dict(cE=n), dict(npag=0), dict(camada=2), dict(camada=-1), dict(Hk=0), dict(hd=8), dict(pag=48), dict(tab=n),
-             dict(comp=n), dict(M=-1), dict(B=0), dict(P=0), dict(novos=-1), dict(teto=65), dict(teto=-1), dict(qm=ctypes.c_void_p((1 << 20) + 4)))
+             dict(comp=n), dict(M=-1), dict(B=0), dict(P=0), dict(novos=-1), dict(teto=2**30), dict(teto=-1), dict(qm=ctypes.c_void_p((1 << 20) + 4)))
     for muda in ruins + (dict(H=-1), dict(H=70000)):
         assert lib.jt_cache_grava(*{**grava, **muda}.values()) == 1, muda
-    nws = lib.jt_atencao_cache_ws_bytes(4, 4, 64, 64, 0, 0)
-    at = dict(qm=p, qE=p, cm=p, cE=p, npag=10, camadas=2, camada=1, Hk=2, hd=64, pag=16, tab=p, comp=p, ini=p, incl=n, out=p, outE=p, M=4, B=2, P=4, novos=2,
-              teto=64, H=4, janela=0, sumid=0, tipo=0, ws=p, nws=ctypes.c_longlong(nws), kid=0)
+    nws = lib.jt_atencao_cache_ws_bytes(4, 2, 4, 2, 64, 2, 8192, 0, 0, 0)
+    at = dict(qm=p, qE=p, cm=p, cE=p, npag=10, camadas=2, camada=1, Hk=2, hd=64, pag=16, tab=p, comp=p, ini=p, incl=n, out=p, outE=p, M=4, B=2, P=512, novos=2,
+              teto=8192, H=4, janela=0, sumid=0, tipo=0, ws=p, nws=ctypes.c_longlong(nws), kid=0)
     assert nws > 0 and lib.jt_atencao_cache(*{**at, "M": 0}.values()) == 0
-    for muda in ruins + (dict(H=3), dict(H=0), dict(out=n), dict(outE=n), dict(janela=-1), dict(sumid=-1), dict(tipo=3), dict(tipo=-1), dict(ws=n),
+    for muda in ruins + (dict(teto=8193), dict(H=3), dict(H=0), dict(out=n), dict(outE=n), dict(janela=-1), dict(sumid=-1), dict(tipo=3), dict(tipo=-1), dict(ws=n),
                          dict(nws=ctypes.c_longlong(nws - 1)), dict(ws=ctypes.c_void_p((1 << 20) + 4))):
         assert lib.jt_atencao_cache(*{**at, **muda}.values()) == 1, muda
     val = dict(m=p, E=p, out=p, n=ctypes.c_longlong(64), cru=0, tipo=1, kid=0)
