@@ -1045,30 +1045,33 @@ int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, in
     return 0;
 }
 
-// How a call runs. mf: several rows share keys and values (k_atc_mf, 64 rows a workgroup, por_seq workgroups a sequence);
-// else a row each (k_atc_um). S splits of the visible tokens, `fatia` tokens (mf: 64-token tiles) each: as many as fill
-// the chip, each with at least one step (um) or 4 tiles (mf) of a workgroup's loop. direto: one split, and every block
-// of the output lies in a head, so the kernel writes it and there is no join.
-struct PlanoAtc { bool mf, direto; int por_seq, S, fatia; };
+// How a call runs, by the rows that share a kv head's keys at most: one (k_atc_um, a row per workgroup), up to 16 (k_atc_gr) or
+// more (k_atc_mf, 64 rows a workgroup, por_seq workgroups a sequence). S splits of the visible tokens, `fatia` tokens (um) or
+// tiles of 32 (gr) or 64 (mf) tokens each: as many as fill the chip, each with at least one step of a workgroup's loop (um), two
+// tiles a wave (gr) or four tiles (mf). direto: one split, and every block of the output lies in a head, so the kernel
+// writes it and there is no join.
+enum { ATC_UM, ATC_GR, ATC_MF };
+struct PlanoAtc { int tipo; bool direto; int por_seq, S, fatia; };
 static PlanoAtc atc_plano(long long M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo) {
     PlanoAtc p;
-    const long long linhas = (long long)novos * (H / Hk);            // that share a kv head's keys, at most
-    p.mf = linhas > 1;
-    p.por_seq = (int)std::max(1LL, (linhas + 63) / 64);
-    long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto), passo, wgs;
-    if (p.mf) {                                                      // in tiles: a window's may begin and end inside one, the first tokens' too
-        const long long nt = (teto + 63LL) / 64;
-        nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, 64LL) + 62) / 64 + 1 + (sumid + 63LL) / 64) : nt);
-        passo = 4;
-        wgs = (long long)B * p.por_seq * Hk;
-    } else {
+    const long long linhas = (long long)novos * (H / Hk);
+    p.tipo = linhas > 16 ? ATC_MF : linhas > 1 ? ATC_GR : ATC_UM;
+    p.por_seq = p.tipo == ATC_MF ? (int)((linhas + 63) / 64) : 1;
+    long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto), passo, wgs, alvo = 2048;
+    if (p.tipo == ATC_UM) {
         passo = hd <= 16 ? 1024 : 16384 / hd;
         wgs = M * H;
+    } else {                                                         // in tiles: a window's may begin and end inside one, the first tokens' too
+        const long long tk = p.tipo == ATC_MF ? 64 : 32, nt = (teto + tk - 1) / tk;
+        nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, 64LL) + tk - 2) / tk + 1 + (sumid + tk - 1) / tk) : nt);
+        passo = p.tipo == ATC_MF ? 4 : 8;
+        if (p.tipo == ATC_MF) alvo = 1024;
+        wgs = (long long)B * p.por_seq * Hk;
     }
-    const long long s = std::min(std::max((p.mf ? 1024 : 2048) / std::max(wgs, 1LL), 1LL), (nv + passo - 1) / passo);
+    const long long s = std::min(std::max(alvo / std::max(wgs, 1LL), 1LL), (nv + passo - 1) / passo);
     p.fatia = (int)(((nv + s - 1) / s + passo - 1) / passo * passo);
     p.S = (int)((nv + p.fatia - 1) / p.fatia);
-    p.direto = p.mf && p.S == 1 && (tipo != 0 || hd >= g_blk);
+    p.direto = p.tipo != ATC_UM && p.S == 1 && (tipo != 0 || hd >= g_blk);
     return p;
 }
 long long jt_atencao_cache_ws_bytes(int M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo) {
@@ -1092,8 +1095,9 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
                       (const float*)incl, ml, po, out, (int8_t*)outE, camadas * camada_m, camadas * camada_e,
                       atc::Lote{(const int*)tab, (const int*)comp, (const int*)ini, B, P, M, ilog2(pag), npag, novos, teto},
                       H, Hk, ilog2(g_blk), janela, sumid, p.S, p.fatia, tipo, kid};
-#define F(HD, GS) (p.mf ? k_atc_mf<HD, GS><<<dim3((B + 1) * p.por_seq, Hk, p.S), 256, 0, g_stream>>>(a, p.por_seq) \
-                        : k_atc_um<HD, GS><<<dim3(M, H, p.S), 256, 0, g_stream>>>(a))
+#define F(HD, GS) (p.tipo == ATC_MF ? k_atc_mf<HD, GS><<<dim3((B + 1) * p.por_seq, Hk, p.S), 256, 0, g_stream>>>(a, p.por_seq) \
+                   : p.tipo == ATC_GR ? k_atc_gr<HD, GS><<<dim3(B + 1, Hk, p.S), 256, 0, g_stream>>>(a) \
+                                      : k_atc_um<HD, GS><<<dim3(M, H, p.S), 256, 0, g_stream>>>(a))
     POR_CABECA(F)
 #undef F
     int rc = fim();

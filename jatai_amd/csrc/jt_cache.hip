@@ -115,7 +115,7 @@ struct Args {
     int8_t* outE;
     long long pag_m, pag_e;
     Lote L;
-    int H, Hk, lgblk, janela, sumid, S, fatia, tipo, kid;   // S splits of `fatia` visible tokens (k_atc_mf: 64-token tiles) each
+    int H, Hk, lgblk, janela, sumid, S, fatia, tipo, kid;   // S splits of `fatia` visible tokens (k_atc_gr, k_atc_mf: tiles) each
 };
 
 // Scores stay in nats (a factor of log2 e would round each of them once more) and become powers of two as
@@ -331,6 +331,253 @@ __global__ void __launch_bounds__(256) k_atc_junta(const float* __restrict__ ml,
     }
 }
 
+namespace atc {
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef int i4_t __attribute__((ext_vector_type(4)));
+constexpr int OCULTA = -2;                       // in place of a page: a key that no row of the workgroup sees
+
+// A row without visible tokens: its outputs (or the marks of its split) for the query heads of kv head hk, by the whole
+// workgroup
+template <int HD>
+__device__ __forceinline__ void vazia(const Args& a, long long r, int hk) {
+    const int Gq = a.H / a.Hk, C = a.H * HD;
+    for (int x = threadIdx.x; x < Gq * HD; x += 256) {
+        const int h = hk * Gq + x / HD;
+        const long long o = r * C + h * HD + x % HD;
+        if (a.ml) {
+            if (x % HD == 0) { float* y = a.ml + 2 * ((r * a.H + h) * a.S + blockIdx.z); y[0] = -INFINITY; y[1] = 0.f; }
+        } else if (a.tipo == 0) {
+            reinterpret_cast<int8_t*>(a.out)[o] = 0;
+            if (!((h * HD + x % HD) & ((1 << a.lgblk) - 1))) a.outE[o >> a.lgblk] = E_ZERO;
+        } else if (a.tipo == 1) reinterpret_cast<__bf16*>(a.out)[o] = (__bf16)0.f;
+        else reinterpret_cast<float*>(a.out)[o] = 0.f;
+    }
+}
+
+// The rows that workgroup (sequence b, tile of `por_wg` rows) has; false: none (rows of no sequence and of a malformed one are
+// zeroed here). b = B: the rows of no sequence, shared out among the tiles.
+template <int HD>
+__device__ __forceinline__ bool linhas_de(const Args& a, int b, int tile, int por_seq, int por_wg, int hk, int& r0, int& n, int& comp) {
+    if (b == a.L.B) {
+        const int ini = a.L.ini ? a.L.ini[0] : 0, fim = a.L.ini ? a.L.ini[a.L.B] : a.L.B;
+        for (long long x = tile; x < min(ini, a.L.M); x += por_seq) vazia<HD>(a, x, hk);
+        for (long long x = max(fim, 0) + (long long)tile; x < a.L.M; x += por_seq) vazia<HD>(a, x, hk);
+        return false;
+    }
+    if (!sequencia(a.L, b, r0, n, comp, a.kid, threadIdx.x == 0 && hk == 0 && blockIdx.z == 0 && tile == 0)) {
+        const long long fim = a.L.ini ? (long long)a.L.ini[b + 1] : b + 1;
+        if (tile == 0)
+            for (long long r = max(r0, 0); r < min(fim, (long long)a.L.M); r++) vazia<HD>(a, r, hk);
+        return false;
+    }
+    if (!a.L.ini && n == 0 && tile == 0 && r0 < a.L.M) vazia<HD>(a, r0, hk);
+    return (long long)tile * por_wg < (long long)n * (a.H / a.Hk);
+}
+
+// The tiles of TK keys that rows at positions i_lo .. i_hi see, numbered without gaps: those of the first tokens, then the
+// window's; and this split's share of them
+template <int TK>
+struct Tiles {
+    int lo, ns, nst, prim, t0, t1;
+    __device__ __forceinline__ Tiles(const Args& a, int i_lo, int i_hi) {
+        lo = a.janela > 0 ? max(0, i_lo + 1 - a.janela) : 0;
+        ns = min(a.sumid, lo);
+        nst = (ns + TK - 1) / TK;
+        prim = max(nst, lo / TK);
+        const int T = nst + i_hi / TK - prim + 1;
+        t0 = min((long long)blockIdx.z * a.fatia, (long long)T);
+        t1 = min(t0 + a.fatia, T);
+    }
+    __device__ __forceinline__ int j0(int t) const { return TK * (t < nst ? t : t - nst + prim); }
+};
+// the page of key j where some row sees it, else OCULTA (also a page outside the cache, which is reported)
+template <class T>
+__device__ __forceinline__ int pagina(const Args& a, const T& tl, int b, int t, int j, int i_hi, bool relata) {
+    const bool vis = t < tl.t1 && j <= i_hi && (j >= tl.lo || j < tl.ns);
+    const int p = a.L.tab[(long long)b * a.L.P + (vis ? j >> a.L.lgpag : 0)];
+    if (!vis) return OCULTA;
+    if ((unsigned)p < (unsigned)a.L.npag) return p;
+    if (relata) reporta(E_ARG, a.kid, (long long)b * a.L.P + (j >> a.L.lgpag), p, j);
+    return OCULTA;
+}
+
+// the bytes 32 k + 8 c .. + 7 of a head row: a lane's share of the k-th MFMA (zeros past the head's width)
+template <int HD>
+__device__ __forceinline__ long fragmento(const int8_t* linha, int k, int c) {
+    if constexpr (HD >= 32) return *reinterpret_cast<const long*>(linha + 32 * k + 8 * c);
+    else if constexpr (HD == 16) return c < 2 ? *reinterpret_cast<const long*>(linha + 8 * c) : 0;
+    else return c == 0 ? (long)*reinterpret_cast<const unsigned*>(linha) : 0;
+}
+
+// A lane's query row: the MFMA operands, the scale of each exponent group, position, bias
+template <int HD, int GS>
+struct Linha {
+    static constexpr int NM = HD < 32 ? 1 : HD / 32, G = HD / GS, MPG = NM / G;      // MFMAs of a score, groups, MFMAs of a group
+    long q[NM];
+    float fq[G], incl;
+    long long r;
+    int h, i;
+    __device__ __forceinline__ Linha(const Args& a, int r0, int n, int comp, int hk, int rho, int c) {
+        const int Gq = a.H / a.Hk, ld = (a.H + 2 * a.Hk) * HD;
+        h = hk * Gq + rho % Gq;
+        i = comp - n + rho / Gq;
+        r = r0 + rho / Gq;
+        incl = a.incl ? a.incl[h] : 0.f;
+#pragma unroll
+        for (int k = 0; k < NM; k++) q[k] = fragmento<HD>(a.qm + r * ld + h * HD, k, c);
+#pragma unroll
+        for (int g = 0; g < G; g++)
+            fq[g] = __builtin_ldexpf(1.f / __builtin_sqrtf((float)HD), a.qE[r * (ld >> a.lgblk) + ((h * HD + g * GS) >> a.lgblk)]);
+    }
+    // scores of 16 keys (kf: their operands; f: 2^Ek per group of this lane's 4 keys 4 c ..), the first of which is j
+    __device__ __forceinline__ void notas(const long (&kf)[NM], const float4 (&f)[G], int j, float* s) const {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            i4_t p = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = g * MPG; k < (g + 1) * MPG; k++) p = __builtin_amdgcn_mfma_i32_16x16x32_i8(kf[k], q[k], p, 0, 0, 0);
+            x[0] += (float)p[0] * f[g].x * fq[g]; x[1] += (float)p[1] * f[g].y * fq[g];
+            x[2] += (float)p[2] * f[g].z * fq[g]; x[3] += (float)p[3] * f[g].w * fq[g];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[k] = x[k] - incl * (float)(i - j - k);
+    }
+    __device__ __forceinline__ bool ve(const Args& a, int j) const { return j <= i && (a.janela <= 0 || j > i - a.janela || j < a.sumid); }
+};
+
+// The running softmax of a lane's row and the outputs it accumulates, O^T tiles of 16 dimensions (lane: row, 4 dimensions)
+template <int HD>
+struct Corrente {
+    static constexpr int DT = HD < 16 ? 1 : HD / 16;
+    float m = -INFINITY, l = 0.f;
+    f4_t o[DT];
+    __device__ __forceinline__ Corrente() {
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = f4_t{0, 0, 0, 0};
+    }
+    // weights of a row's scores s (4 keys of every 16 in a lane) as three bf16 pieces, 24 bits, exactly
+    template <int N>
+    __device__ __forceinline__ void pesos(const float (&s)[N], i4_t (&p)[3][N / 8]) {
+        float mx = s[0];
+#pragma unroll
+        for (int k = 1; k < N; k++) mx = fmaxf(mx, s[k]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        if (__any(mx > m + 5.f)) {
+            const float mn = fmaxf(m, mx), al = fator(m, mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= al;
+        }
+        const float mL = m == -INFINITY ? 0.f : vezes_log2e(m);
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            int y[3][2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const float e = peso(s[k + x], mL);
+                l += e;
+                y[0][x] = __float_as_int(e);
+                const float e1 = e - __int_as_float(y[0][x] & 0xffff0000);
+                y[1][x] = __float_as_int(e1);
+                y[2][x] = __float_as_int(e1 - __int_as_float(y[1][x] & 0xffff0000));
+            }
+#pragma unroll
+            for (int x = 0; x < 3; x++) p[x][k / 8][k % 8 / 2] = (int)__builtin_amdgcn_perm((unsigned)y[x][1], (unsigned)y[x][0], 0x07060302u);
+        }
+    }
+    // O^T += V^T P^T over 32 keys, whose values are the rows of v in LDS (VS bf16 each)
+    template <int VS>
+    __device__ __forceinline__ void soma_v(const __bf16* v, const i4_t& p0, const i4_t& p1, const i4_t& p2, int lr, int c) {
+        typedef __attribute__((address_space(3))) s4_t* lds4;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            // lane 16 c + x reads row 4 c + x / 4, columns 4 (x % 4) ..; it receives column x of the 4 rows
+            const __bf16* y = v + (4 * c + lr / 4) * VS + 16 * d + 4 * (lr % 4);
+            const s4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(y)), v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(y + 16 * VS));
+            const b8_t x = __builtin_bit_cast(b8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(b8_t, p0), o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(b8_t, p1), o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(b8_t, p2), o[d], 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void soma_l() {
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+    }
+    // the row's partial result, or its output
+    template <int GS>
+    __device__ __forceinline__ void grava(const Args& a, long long r, int h, int c) {
+        const int C = a.H * HD;
+        if (a.ml) {
+            const long long part = (r * a.H + h) * a.S + blockIdx.z;
+            if (c == 0) { a.ml[2 * part] = m; a.ml[2 * part + 1] = l; }
+            if (HD >= 16 || c == 0)
+#pragma unroll
+                for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(a.o + part * HD + 16 * d + 4 * c) = o[d];
+            return;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] *= inv;
+        const long long x = r * C + h * HD;
+        if (a.tipo == 0) {                                            // blocks lie in the head (a plan's `direto`): GS = BLK
+            if constexpr (HD >= 32) {
+                constexpr int G = HD / GS, DG = DT / G;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    int bits = 0;
+#pragma unroll
+                    for (int d = 0; d < 4 * DG; d++) bits = max(bits, __float_as_int(o[g * DG + d / 4][d % 4]) & 0x7fffffff);
+                    bits = max(bits, __shfl_xor(bits, 16));
+                    bits = max(bits, __shfl_xor(bits, 32));
+                    float f;
+                    const int E = expoente_f32(bits, f, a.kid, x + g * GS);
+#pragma unroll
+                    for (int d = g * DG; d < (g + 1) * DG; d++) {
+                        int8_t z[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) z[k] = E == E_ZERO ? 0 : (int8_t)(int)__builtin_rintf(o[d][k] * f);
+                        grava_i8<4, false>((int8_t*)a.out + x + 16 * d + 4 * c, z);
+                    }
+                    if (c == 0) a.outE[(x >> a.lgblk) + g] = (int8_t)E;
+                }
+            }
+        } else if (HD >= 16 || c == 0) {
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                typedef __bf16 b4_t __attribute__((ext_vector_type(4)));
+                if (a.tipo == 1) *reinterpret_cast<b4_t*>((__bf16*)a.out + x + 16 * d + 4 * c) = b4_t{(__bf16)o[d][0], (__bf16)o[d][1], (__bf16)o[d][2], (__bf16)o[d][3]};
+                else *reinterpret_cast<f4_t*>((float*)a.out + x + 16 * d + 4 * c) = o[d];
+            }
+        }
+    }
+};
+
+// VB mantissas of a value and its exponent, into a row of bf16 in LDS: m 2^E is exact there. A row narrower than 16 is
+// filled up with zeros.
+template <int VB>
+__device__ __forceinline__ void valor_lds(__bf16* p, const int4& d, float e) {
+    const int y[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int k = 0; k < 16; k += 8) {
+        b8_t z;
+#pragma unroll
+        for (int x = 0; x < 8; x++) z[x] = (__bf16)(k + x < VB ? e * (float)(int8_t)(y[(k + x) / 4] >> (8 * (x % 4))) : 0.f);
+        *reinterpret_cast<b8_t*>(p + k) = z;
+    }
+}
+template <int VB>
+__device__ __forceinline__ int4 le_vb(const int8_t* p) {
+    if constexpr (VB == 16) return *reinterpret_cast<const int4*>(p);
+    else return make_int4(*reinterpret_cast<const int*>(p), 0, 0, 0);
+}
+}  // namespace atc
+
 // Several rows that share keys and values (new tokens of a sequence, query heads of a group): 64 of them per workgroup, 16 a
 // wave, on matrix cores; the workgroup walks its keys in tiles of 64. Row rho of a (sequence, kv head) is token rho / Gq,
 // head rho % Gq of the group.
@@ -343,93 +590,31 @@ __global__ void __launch_bounds__(256) k_atc_junta(const float* __restrict__ ml,
 // raised (and O rescaled) only where a tile exceeds it by 5 nats: weights are then at most e^5, which costs fp32 no precision.
 template <int HD, int GS>
 __global__ void __launch_bounds__(256) k_atc_mf(atc::Args a, int por_seq) {
-    typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
-    typedef short s4_t __attribute__((ext_vector_type(4)));
-    typedef float f4_t __attribute__((ext_vector_type(4)));
-    typedef int i4_t __attribute__((ext_vector_type(4)));
-    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 64;
-    constexpr int NM = HD < 32 ? 1 : HD / 32, MPG = NM / G, DT = HD < 16 ? 1 : HD / 16;       // MFMAs of a score, per group; tiles of O
-    constexpr int KS = HD < 16 ? 4 : HD + 8, VS = 16 * DT + 8;                                // LDS rows, in values
+    using namespace atc;
+    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 64, NM = Linha<HD, GS>::NM;
+    constexpr int KS = HD < 16 ? 4 : HD + 8, VS = 16 * Corrente<HD>::DT + 8;                  // LDS rows, in values
     constexpr int NT = 2 * TK * LPK, IT = (NT + 255) / 256, NK = IT == 4 ? 2 : 1;             // staging: tasks, per thread; keys of a thread
     __shared__ __align__(16) int8_t sk[2][TK * KS];
     __shared__ __align__(16) __bf16 sv[2][TK * VS];
     __shared__ __align__(16) float sf[2][G * TK];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk, C = a.H * HD;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk;
     const int b = blockIdx.x / por_seq, tile = por_seq - 1 - blockIdx.x % por_seq;            // a sequence's last rows, the longest, first
-
-    // a row without visible tokens: its outputs (or the marks of its splits) for this workgroup's heads
-    auto vazia = [&](long long r) {
-        for (int x = threadIdx.x; x < Gq * HD; x += 256) {
-            const int h = hk * Gq + x / HD;
-            const long long o = r * C + h * HD + x % HD;
-            if (a.ml) {
-                if (x % HD == 0) { float* y = a.ml + 2 * ((r * a.H + h) * a.S + blockIdx.z); y[0] = -INFINITY; y[1] = 0.f; }
-            } else if (a.tipo == 0) {
-                reinterpret_cast<int8_t*>(a.out)[o] = 0;
-                if (!((h * HD + x % HD) & ((1 << a.lgblk) - 1))) a.outE[o >> a.lgblk] = E_ZERO;
-            } else if (a.tipo == 1) reinterpret_cast<__bf16*>(a.out)[o] = (__bf16)0.f;
-            else reinterpret_cast<float*>(a.out)[o] = 0.f;
-        }
-    };
-    if (b == a.L.B) {                                                 // rows of no sequence
-        const int ini = a.L.ini ? a.L.ini[0] : 0, fim = a.L.ini ? a.L.ini[a.L.B] : a.L.B;
-        for (long long x = tile; x < min(ini, a.L.M); x += por_seq) vazia(x);
-        for (long long x = max(fim, 0) + (long long)tile; x < a.L.M; x += por_seq) vazia(x);
-        return;
-    }
     int r0, n, comp;
-    if (!atc::sequencia(a.L, b, r0, n, comp, a.kid, threadIdx.x == 0 && hk == 0 && blockIdx.z == 0 && tile == 0)) {
-        const long long fim = a.L.ini ? (long long)a.L.ini[b + 1] : b + 1;
-        if (tile == 0)
-            for (long long r = max(r0, 0); r < min(fim, (long long)a.L.M); r++) vazia(r);
-        return;
-    }
-    if (!a.L.ini && n == 0 && tile == 0 && r0 < a.L.M) vazia(r0);
-    const int linhas = n * Gq, rho0 = tile * 64;
-    if (rho0 >= linhas) return;
-    const int i_lo = comp - n + rho0 / Gq, i_hi = comp - n + min(rho0 + 63, linhas - 1) / Gq;
-    const int lo = a.janela > 0 ? max(0, i_lo + 1 - a.janela) : 0, ns = min(a.sumid, lo), nst = (ns + TK - 1) / TK, prim = max(nst, lo / TK);
-    const int T = nst + i_hi / TK - prim + 1, t0 = min((long long)blockIdx.z * a.fatia, (long long)T), t1 = min(t0 + a.fatia, T);
-
-    // this lane's row
-    const int rho = rho0 + 16 * w + lr, rc = min(rho, linhas - 1), h = hk * Gq + rc % Gq, i = comp - n + rc / Gq;
-    const int w_hi = comp - n + min(rho0 + 16 * w + 15, linhas - 1) / Gq;                     // the wave's last position
+    if (!linhas_de<HD>(a, b, tile, por_seq, 64, hk, r0, n, comp)) return;
+    const int linhas = n * Gq, rho0 = tile * 64, i_lo = comp - n + rho0 / Gq, i_hi = comp - n + min(rho0 + 63, linhas - 1) / Gq;
+    const Tiles<TK> tl(a, i_lo, i_hi);
+    const int rho = rho0 + 16 * w + lr, w_hi = comp - n + min(rho0 + 16 * w + 15, linhas - 1) / Gq;   // w_hi: the wave's last position
     const bool tem = rho0 + 16 * w < linhas;
-    const long long r = r0 + rc / Gq;
-    const int ld = (a.H + 2 * a.Hk) * HD;
-    const float incl = a.incl ? a.incl[h] : 0.f;
-    long q[NM];
-    float fq[G];
-#pragma unroll
-    for (int k = 0; k < NM; k++) {
-        const int8_t* p = a.qm + r * ld + h * HD + 32 * k + 8 * c;
-        if constexpr (HD >= 32) q[k] = *reinterpret_cast<const long*>(p);
-        else if constexpr (HD == 16) q[k] = c < 2 ? *reinterpret_cast<const long*>(p) : 0;
-        else q[k] = c == 0 ? (long)*reinterpret_cast<const unsigned*>(p) : 0;
-    }
-#pragma unroll
-    for (int g = 0; g < G; g++)
-        fq[g] = __builtin_ldexpf(1.f / __builtin_sqrtf((float)HD), a.qE[r * (ld >> a.lgblk) + ((h * HD + g * GS) >> a.lgblk)]);
+    const Linha<HD, GS> q(a, r0, n, comp, hk, min(rho, linhas - 1), c);
 
     const int pag = 1 << a.L.lgpag;
-    auto j0_de = [&](int t) { return TK * (t < nst ? t : t - nst + prim); };
-    constexpr int OCULTA = -2;                                        // a key that no row of the workgroup sees
     int pg[NK];
     int4 dm[IT];
     int de[IT];
     auto chave = [&](int k) { return (int)((threadIdx.x / LPK + 32 * k) % TK); };
     auto le_paginas = [&](int t) {
 #pragma unroll
-        for (int k = 0; k < NK; k++) {
-            const int j = j0_de(t) + chave(k);
-            const bool vis = t < t1 && j <= i_hi && (j >= lo || j < ns);
-            const int p = a.L.tab[(long long)b * a.L.P + (vis ? j >> a.L.lgpag : 0)];
-            pg[k] = vis ? p : OCULTA;
-            if (vis && (unsigned)p >= (unsigned)a.L.npag) {
-                if (hk == 0 && threadIdx.x % LPK == 0) reporta(E_ARG, a.kid, (long long)b * a.L.P + (j >> a.L.lgpag), p, j);
-                pg[k] = OCULTA;
-            }
-        }
+        for (int k = 0; k < NK; k++) pg[k] = pagina(a, tl, b, t, tl.j0(t) + chave(k), i_hi, hk == 0 && threadIdx.x % LPK == 0);
     };
     // task: a chunk of VB bytes of a key (first TK LPK tasks) or a value, and its exponent
     auto le_dados = [&](int t) {
@@ -439,10 +624,8 @@ __global__ void __launch_bounds__(256) k_atc_mf(atc::Args a, int por_seq) {
             dm[x] = make_int4(0, 0, 0, 0);
             de[x] = -127;
             if (tarefa < NT && pg[k] != OCULTA) {
-                const long long vaga = ((long long)kv * a.Hk + hk) * pag + ((j0_de(t) + chave(k)) & (pag - 1));
-                const int8_t* p = a.cm + pg[k] * a.pag_m + vaga * HD + cc * VB;
-                if constexpr (VB == 16) dm[x] = *reinterpret_cast<const int4*>(p);
-                else dm[x].x = *reinterpret_cast<const int*>(p);
+                const long long vaga = ((long long)kv * a.Hk + hk) * pag + ((tl.j0(t) + chave(k)) & (pag - 1));
+                dm[x] = le_vb<VB>(a.cm + pg[k] * a.pag_m + vaga * HD + cc * VB);
                 de[x] = a.cE[pg[k] * a.pag_e + vaga * G + cc * VB / GS];
             }
         }
@@ -460,160 +643,179 @@ __global__ void __launch_bounds__(256) k_atc_mf(atc::Args a, int por_seq) {
                     reinterpret_cast<int2*>(p)[1] = make_int2(dm[x].z, dm[x].w);
                 } else *reinterpret_cast<int*>(p) = dm[x].x;
                 if (cc * VB % GS == 0) sf[buf][cc * VB / GS * TK + key] = e;
-            } else {
-                const int y[4] = {dm[x].x, dm[x].y, dm[x].z, dm[x].w};
-                __bf16* p = &sv[buf][key * VS + cc * VB];
-#pragma unroll
-                for (int d = 0; d < VB; d += 8) {
-                    b8_t z;
-#pragma unroll
-                    for (int k8 = 0; k8 < 8; k8++) z[k8] = (__bf16)(d + k8 < VB ? e * (float)(int8_t)(y[(d + k8) / 4 % 4] >> (8 * (k8 % 4))) : 0.f);
-                    *reinterpret_cast<b8_t*>(p + d) = z;
-                }
-                if constexpr (HD < 16) *reinterpret_cast<b8_t*>(p + 8) = b8_t{};
-            }
+            } else valor_lds<VB>(&sv[buf][key * VS + cc * VB], dm[x], e);
         }
     };
 
-    float m = -INFINITY, l = 0.f;
-    f4_t o[DT];
-#pragma unroll
-    for (int d = 0; d < DT; d++) o[d] = f4_t{0, 0, 0, 0};
-    if (t0 < t1) {
-        le_paginas(t0);
-        le_dados(t0);
-        le_paginas(t0 + 1);
+    Corrente<HD> y;
+    if (tl.t0 < tl.t1) {
+        le_paginas(tl.t0);
+        le_dados(tl.t0);
+        le_paginas(tl.t0 + 1);
         guarda(0);
     }
     __syncthreads();
-    for (int t = t0; t < t1; t++) {
-        const int buf = (t - t0) & 1, j0 = j0_de(t);
-        if (t + 1 < t1) { le_dados(t + 1); le_paginas(t + 2); }
+    for (int t = tl.t0; t < tl.t1; t++) {
+        const int buf = (t - tl.t0) & 1, j0 = tl.j0(t);
+        if (t + 1 < tl.t1) { le_dados(t + 1); le_paginas(t + 2); }
         if (tem && j0 <= w_hi) {
             float s[16];
 #pragma unroll
             for (int kt = 0; kt < 4; kt++) {
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                long kf[NM];
+                float4 f[G];
 #pragma unroll
-                for (int g = 0; g < G; g++) {
-                    i4_t p = {0, 0, 0, 0};
+                for (int k = 0; k < NM; k++) kf[k] = fragmento<HD>(&sk[buf][(16 * kt + lr) * KS], k, c);
 #pragma unroll
-                    for (int k = g * MPG; k < (g + 1) * MPG; k++) {
-                        const int8_t* y = &sk[buf][(16 * kt + lr) * KS + 32 * k + 8 * c];
-                        long kf;
-                        if constexpr (HD >= 32) kf = *reinterpret_cast<const long*>(y);
-                        else if constexpr (HD == 16) kf = c < 2 ? *reinterpret_cast<const long*>(y) : 0;
-                        else kf = c == 0 ? (long)*reinterpret_cast<const unsigned*>(y) : 0;
-                        p = __builtin_amdgcn_mfma_i32_16x16x32_i8(kf, q[k], p, 0, 0, 0);
-                    }
-                    const float4 f = *reinterpret_cast<const float4*>(&sf[buf][g * TK + 16 * kt + 4 * c]);
-                    x[0] += (float)p[0] * f.x * fq[g]; x[1] += (float)p[1] * f.y * fq[g];
-                    x[2] += (float)p[2] * f.z * fq[g]; x[3] += (float)p[3] * f.w * fq[g];
-                }
-#pragma unroll
-                for (int k = 0; k < 4; k++) s[4 * kt + k] = x[k] - incl * (float)(i - j0 - 16 * kt - 4 * c - k);
+                for (int g = 0; g < G; g++) f[g] = *reinterpret_cast<const float4*>(&sf[buf][g * TK + 16 * kt + 4 * c]);
+                q.notas(kf, f, j0 + 16 * kt + 4 * c, s + 4 * kt);
             }
             // every key of the tile visible to every row of the workgroup: nothing to mask
             if (j0 + TK - 1 > i_lo || (a.janela > 0 && j0 <= i_hi - a.janela && j0 + TK > a.sumid)) {
 #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const int j = j0 + 16 * (k / 4) + 4 * c + k % 4;
-                    const bool vis = j <= i && (a.janela <= 0 || j > i - a.janela || j < a.sumid);
-                    s[k] = vis ? s[k] : -INFINITY;
-                }
+                for (int k = 0; k < 16; k++) s[k] = q.ve(a, j0 + 16 * (k / 4) + 4 * c + k % 4) ? s[k] : -INFINITY;
             }
-            float mx = s[0];
+            i4_t p[3][2];
+            y.pesos(s, p);
 #pragma unroll
-            for (int k = 1; k < 16; k++) mx = fmaxf(mx, s[k]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            if (__any(mx > m + 5.f)) {
-                const float mn = fmaxf(m, mx), al = atc::fator(m, mn);
-                m = mn;
-                l *= al;
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[d] *= al;
-            }
-            const float mL = m == -INFINITY ? 0.f : atc::vezes_log2e(m);
-            i4_t p[3][2];                                             // a weight's 24 bits in three bf16 pieces, exactly
-#pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-                int y[3][2];
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const float e = atc::peso(s[k + x], mL);
-                    l += e;
-                    y[0][x] = __float_as_int(e);
-                    const float e1 = e - __int_as_float(y[0][x] & 0xffff0000);
-                    y[1][x] = __float_as_int(e1);
-                    y[2][x] = __float_as_int(e1 - __int_as_float(y[1][x] & 0xffff0000));
-                }
-#pragma unroll
-                for (int x = 0; x < 3; x++) p[x][k / 8][k % 8 / 2] = (int)__builtin_amdgcn_perm((unsigned)y[x][1], (unsigned)y[x][0], 0x07060302u);
-            }
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    // lane 16 c + x reads row 4 c + x / 4, columns 4 (x % 4) ..; it receives column x of the 4 rows
-                    const __bf16* y = &sv[buf][(32 * kk + 4 * c + lr / 4) * VS + 16 * d + 4 * (lr % 4)];
-                    typedef __attribute__((address_space(3))) s4_t* lds4;
-                    const s4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(y)), v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(y + 16 * VS));
-                    const b8_t v = __builtin_bit_cast(b8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int x = 0; x < 3; x++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(b8_t, p[x][kk]), o[d], 0, 0, 0);
-                }
+            for (int kk = 0; kk < 2; kk++) y.template soma_v<VS>(&sv[buf][32 * kk * VS], p[0][kk], p[1][kk], p[2][kk], lr, c);
         }
-        if (t + 1 < t1) guarda(buf ^ 1);
+        if (t + 1 < tl.t1) guarda(buf ^ 1);
         __syncthreads();
     }
     if (rho >= linhas) return;
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (a.ml) {
-        const long long part = (r * a.H + h) * a.S + blockIdx.z;
-        if (c == 0) { a.ml[2 * part] = m; a.ml[2 * part + 1] = l; }
-        if (HD >= 16 || c == 0)
-#pragma unroll
-            for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(a.o + part * HD + 16 * d + 4 * c) = o[d];
-        return;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int d = 0; d < DT; d++) o[d] *= inv;
-    const long long x = r * C + h * HD;
-    if (a.tipo == 0) {                                                // one block of the head's: GS = BLK here
-        if constexpr (HD >= 32) {
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                constexpr int DG = DT / G;
-                int bits = 0;
-#pragma unroll
-                for (int d = 0; d < 4 * DG; d++) bits = max(bits, __float_as_int(o[g * DG + d / 4][d % 4]) & 0x7fffffff);
-                bits = max(bits, __shfl_xor(bits, 16));
-                bits = max(bits, __shfl_xor(bits, 32));
-                float f;
-                const int E = expoente_f32(bits, f, a.kid, x + g * GS);
-#pragma unroll
-                for (int d = g * DG; d < (g + 1) * DG; d++) {
-                    int8_t z[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) z[k] = E == E_ZERO ? 0 : (int8_t)(int)__builtin_rintf(o[d][k] * f);
-                    grava_i8<4, false>((int8_t*)a.out + x + 16 * d + 4 * c, z);
-                }
-                if (c == 0) a.outE[(x >> a.lgblk) + g] = (int8_t)E;
-            }
-        }
-    } else if (HD >= 16 || c == 0) {
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            typedef __bf16 b4_t __attribute__((ext_vector_type(4)));
-            if (a.tipo == 1) *reinterpret_cast<b4_t*>((__bf16*)a.out + x + 16 * d + 4 * c) = b4_t{(__bf16)o[d][0], (__bf16)o[d][1], (__bf16)o[d][2], (__bf16)o[d][3]};
-            else *reinterpret_cast<f4_t*>((float*)a.out + x + 16 * d + 4 * c) = o[d];
-        }
-    }
+    y.soma_l();
+    y.template grava<GS>(a, q.r, q.h, c);
 }
 
+// Up to 16 rows that share keys and values (a new token's query heads of a group, a few new tokens): the same products, but the
+// four waves of a workgroup take every fourth tile of 32 keys for the same rows, without a barrier. A wave reads its keys
+// from memory in the MFMA's own layout, passes its values through its own LDS to transpose them, and has the next
+// tile's bytes in flight while it computes this one. The waves' results are joined at the end. Reading the keys bounds it.
+template <int HD, int GS>
+__global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
+    using namespace atc;
+    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 32, NM = Linha<HD, GS>::NM, DT = Corrente<HD>::DT;
+    constexpr int VS = 16 * DT + 8, IT = (TK * LPK + 63) / 64;
+    constexpr int BV = TK * VS * 2, BF = G * TK * 4, BO = 3 * DT * 64 * 16, BYTES = 4 * (BV + BF) > BO ? 4 * (BV + BF) : BO;
+    __shared__ __align__(16) char mem[BYTES];                         // per wave: values, key scales; at the end the waves' outputs
+    __shared__ float sm[4][16], sl[4][16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk;
+    __bf16* sv = reinterpret_cast<__bf16*>(mem + w * (BV + BF));
+    float* sf = reinterpret_cast<float*>(mem + w * (BV + BF) + BV);
+    int r0, n, comp;
+    if (!linhas_de<HD>(a, blockIdx.x, 0, 1, 16, hk, r0, n, comp)) return;
+    const int b = blockIdx.x, linhas = n * Gq, i_lo = comp - n, i_hi = comp - 1, pag = 1 << a.L.lgpag;
+    const Tiles<TK> tl(a, i_lo, i_hi);
+    const Linha<HD, GS> q(a, r0, n, comp, hk, min(lr, linhas - 1), c);
+
+    // a lane's keys: lr and 16 + lr of the tile for the products; lane / LPK, then 64 / LPK further on, for the values
+    int pk[2], pv[IT], ke[2];
+    long kf[2][NM];
+    int4 dv[IT];
+    int ve[IT];
+    auto le_paginas = [&](int t) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) pk[k] = pagina(a, tl, b, t, tl.j0(t) + 16 * k + lr, i_hi, hk == 0 && c == 0);
+#pragma unroll
+        for (int x = 0; x < IT; x++) {
+            const int key = lane / LPK + 64 / LPK * x;
+            pv[x] = key < TK ? pagina(a, tl, b, t, tl.j0(t) + key, i_hi, false) : OCULTA;
+        }
+    };
+    auto le_dados = [&](int t) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+#pragma unroll
+            for (int x = 0; x < NM; x++) kf[k][x] = 0;
+            ke[k] = -127;
+            if (pk[k] != OCULTA) {
+                const long long vaga = (long long)hk * pag + ((tl.j0(t) + 16 * k + lr) & (pag - 1));
+                const int8_t* p = a.cm + pk[k] * a.pag_m + vaga * HD;
+#pragma unroll
+                for (int x = 0; x < NM; x++) kf[k][x] = fragmento<HD>(p, x, c);
+                if (c < G) ke[k] = a.cE[pk[k] * a.pag_e + vaga * G + c];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < IT; x++) {
+            const int key = lane / LPK + 64 / LPK * x, cc = lane % LPK;
+            dv[x] = make_int4(0, 0, 0, 0);
+            ve[x] = -127;
+            if (pv[x] != OCULTA) {
+                const long long vaga = ((long long)a.Hk + hk) * pag + ((tl.j0(t) + key) & (pag - 1));
+                dv[x] = le_vb<VB>(a.cm + pv[x] * a.pag_m + vaga * HD + cc * VB);
+                ve[x] = a.cE[pv[x] * a.pag_e + vaga * G + cc * VB / GS];
+            }
+        }
+    };
+
+    Corrente<HD> y;
+    int t = tl.t0 + w;
+    if (t < tl.t1) {
+        le_paginas(t);
+        le_dados(t);
+        le_paginas(t + 4);
+    }
+    for (; t < tl.t1; t += 4) {
+        const int j0 = tl.j0(t);
+        long k0[2][NM];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (c < G) sf[c * TK + 16 * k + lr] = __builtin_ldexpf(1.f, ke[k]);
+#pragma unroll
+            for (int x = 0; x < NM; x++) k0[k][x] = kf[k][x];
+        }
+#pragma unroll
+        for (int x = 0; x < IT; x++) {
+            const int key = lane / LPK + 64 / LPK * x;
+            if (key < TK) valor_lds<VB>(sv + key * VS + lane % LPK * VB, dv[x], __builtin_ldexpf(1.f, ve[x]));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (t + 4 < tl.t1) { le_dados(t + 4); le_paginas(t + 8); }
+        float s[8];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            float4 f[G];
+#pragma unroll
+            for (int g = 0; g < G; g++) f[g] = *reinterpret_cast<const float4*>(sf + g * TK + 16 * k + 4 * c);
+            q.notas(k0[k], f, j0 + 16 * k + 4 * c, s + 4 * k);
+        }
+        if (j0 + TK - 1 > i_lo || (a.janela > 0 && j0 <= i_hi - a.janela && j0 + TK > a.sumid)) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) s[k] = q.ve(a, j0 + 16 * (k / 4) + 4 * c + k % 4) ? s[k] : -INFINITY;
+        }
+        i4_t p[3][1];
+        y.pesos(s, p);
+        y.template soma_v<VS>(sv, p[0][0], p[1][0], p[2][0], lr, c);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    // the four waves' results: a common maximum, then sums
+    y.soma_l();
+    if (c == 0) { sm[w][lr] = y.m; sl[w][lr] = y.l; }
+    __syncthreads();
+    float M = sm[0][lr], L = 0.f;
+#pragma unroll
+    for (int k = 1; k < 4; k++) M = fmaxf(M, sm[k][lr]);
+#pragma unroll
+    for (int k = 0; k < 4; k++) L += sl[k][lr] * fator(sm[k][lr], M);
+    const float f = fator(y.m, M);
+    f4_t* so = reinterpret_cast<f4_t*>(mem);
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+        y.o[d] *= f;
+        if (w > 0) so[((w - 1) * DT + d) * 64 + lane] = y.o[d];
+    }
+    __syncthreads();
+    if (w > 0 || lr >= linhas) return;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int k = 0; k < 3; k++) y.o[d] += so[(k * DT + d) * 64 + lane];
+    y.m = M;
+    y.l = L;
+    y.template grava<GS>(a, q.r, q.h, c);
+}
 
 // ---------------------------------------------------------------------------------------------- values
 // A block or raw tensor as floats (the inverse of de_f32), each value rounded once: block values are exact in both types
