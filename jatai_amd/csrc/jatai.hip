@@ -1046,29 +1046,34 @@ int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, in
 }
 
 // How a call runs, by the rows that share a kv head's keys at most: one (k_atc_um, a row per workgroup), up to 16 (k_atc_gr) or
-// more (k_atc_mf, 64 rows a workgroup, por_seq workgroups a sequence). S splits of the visible tokens, `fatia` tokens (um) or
+// more (k_atc_mf, 16 ATC_NW rows a workgroup, por_seq workgroups a sequence). S splits of the visible tokens, `fatia` tokens (um) or
 // tiles of 32 (gr) or 64 (mf) tokens each: as many as fill the chip, each with at least one step of a workgroup's loop (um), two
 // tiles a wave (gr) or four tiles (mf). direto: one split, and every block of the output lies in a head, so the kernel
 // writes it and there is no join.
 enum { ATC_UM, ATC_GR, ATC_MF };
+#ifndef ATC_FATIA
+#define ATC_FATIA 24
+#endif
+constexpr int ATC_NW = 4;                                            // waves of a k_atc_mf workgroup
 struct PlanoAtc { int tipo; bool direto; int por_seq, S, fatia; };
 static PlanoAtc atc_plano(long long M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo) {
     PlanoAtc p;
     const long long linhas = (long long)novos * (H / Hk);
     p.tipo = linhas > 16 ? ATC_MF : linhas > 1 ? ATC_GR : ATC_UM;
-    p.por_seq = p.tipo == ATC_MF ? (int)((linhas + 63) / 64) : 1;
+    p.por_seq = p.tipo == ATC_MF ? (int)((linhas + 16 * ATC_NW - 1) / (16 * ATC_NW)) : 1;
     long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto), passo, wgs, alvo = 2048;
     if (p.tipo == ATC_UM) {
         passo = hd <= 16 ? 1024 : 16384 / hd;
         wgs = M * H;
     } else {                                                         // in tiles: a window's may begin and end inside one, the first tokens' too
         const long long tk = p.tipo == ATC_MF ? 64 : 32, nt = (teto + tk - 1) / tk;
-        nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, 64LL) + tk - 2) / tk + 1 + (sumid + tk - 1) / tk) : nt);
+        nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, 16LL * ATC_NW) + tk - 2) / tk + 1 + (sumid + tk - 1) / tk) : nt);
         passo = p.tipo == ATC_MF ? 4 : 8;
         if (p.tipo == ATC_MF) alvo = 1024;
         wgs = (long long)B * p.por_seq * Hk;
     }
-    const long long s = std::min(std::max(alvo / std::max(wgs, 1LL), 1LL), (nv + passo - 1) / passo);
+    long long s = std::min(std::max(alvo / std::max(wgs, 1LL), 1LL), (nv + passo - 1) / passo);
+    if (p.tipo == ATC_MF) s = std::max(s, (nv + ATC_FATIA - 1) / ATC_FATIA);
     p.fatia = (int)(((nv + s - 1) / s + passo - 1) / passo * passo);
     p.S = (int)((nv + p.fatia - 1) / p.fatia);
     p.direto = p.tipo != ATC_UM && p.S == 1 && (tipo != 0 || hd >= g_blk);
@@ -1094,8 +1099,8 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
     const atc::Args a{(const int8_t*)qm, (const int8_t*)qE, (const int8_t*)cm + camada * camada_m, (const int8_t*)cE + camada * camada_e,
                       (const float*)incl, ml, po, out, (int8_t*)outE, camadas * camada_m, camadas * camada_e,
                       atc::Lote{(const int*)tab, (const int*)comp, (const int*)ini, B, P, M, ilog2(pag), npag, novos, teto},
-                      H, Hk, ilog2(g_blk), janela, sumid, p.S, p.fatia, tipo, kid};
-#define F(HD, GS) (p.tipo == ATC_MF ? k_atc_mf<HD, GS><<<dim3((B + 1) * p.por_seq, Hk, p.S), 256, 0, g_stream>>>(a, p.por_seq) \
+                      tipo != 0 || hd >= g_blk, H, Hk, ilog2(g_blk), janela, sumid, p.S, p.fatia, tipo, kid};
+#define F(HD, GS) (p.tipo == ATC_MF ? k_atc_mf<HD, GS, ATC_NW><<<dim3((B + 1) * p.por_seq, Hk, p.S), 64 * ATC_NW, 0, g_stream>>>(a, p.por_seq) \
                    : p.tipo == ATC_GR ? k_atc_gr<HD, GS><<<dim3(B + 1, Hk, p.S), 256, 0, g_stream>>>(a) \
                                       : k_atc_um<HD, GS><<<dim3(M, H, p.S), 256, 0, g_stream>>>(a))
     POR_CABECA(F)

@@ -115,21 +115,30 @@ struct Args {
     int8_t* outE;
     long long pag_m, pag_e;
     Lote L;
+    bool inteira;                                // the blocks of a block output lie in one head each
     int H, Hk, lgblk, janela, sumid, S, fatia, tipo, kid;   // S splits of `fatia` visible tokens (k_atc_gr, k_atc_mf: tiles) each
 };
+
+// a page outside the cache that the token at position `ruim` (-1: none) of sequence b needed
+__device__ __forceinline__ void relata_pagina(const Args& a, int b, int ruim) {
+    if (ruim < 0) return;
+    const long long x = (long long)b * a.L.P + (ruim >> a.L.lgpag);
+    reporta(E_ARG, a.kid, x, a.L.tab[x], ruim);
+}
 
 // Scores stay in nats (a factor of log2 e would round each of them once more) and become powers of two as
 // exp2(s log2 e - m log2 e), one FMA whose rounding is small where the weight is large. The rounding of m log2 e is common to
 // all weights under a maximum, and the factor between two maxima takes the same rounded products (never contracted into an FMA), so that
 // it fits them, and is exactly 1 where the maximum stays.
+// k_atc_mf keeps scores times sqrt(hd), K then being log2 e / sqrt(hd).
 constexpr float LOG2E = 1.4426950408889634f;
-__device__ __forceinline__ float vezes_log2e(float m) {
+__device__ __forceinline__ float vezes(float m, float K) {
 #pragma clang fp contract(off)
-    return m * LOG2E;
+    return m * K;
 }
-__device__ __forceinline__ float peso(float s, float mL) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, LOG2E, -mL)); }
-// 2^(m log2 e - M log2 e) for m <= M, 0 where m is -inf (also M)
-__device__ __forceinline__ float fator(float m, float M) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(vezes_log2e(m) - vezes_log2e(M)); }
+__device__ __forceinline__ float peso(float s, float mL, float K = LOG2E) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, K, -mL)); }
+// 2^(m K - M K) for m <= M, 0 where m is -inf (also M)
+__device__ __forceinline__ float fator(float m, float M, float K = LOG2E) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(vezes(m, K) - vezes(M, K)); }
 
 template <int LPK>
 __device__ __forceinline__ float soma_grupo(float v) {               // over LPK consecutive lanes, to all of them
@@ -174,6 +183,7 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
 #pragma unroll
     for (int d = 0; d < VB; d++) o[d] = 0.f;
     const long long dv = (long long)a.Hk * pag;                        // slots between a token's key and its value
+    int ruim = -1;
     for (int base = x0 + w * KPW * U; base < x1; base += NW * KPW * U) {
         int j[U], p[U];
         bool vis[U];
@@ -187,11 +197,10 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
         int kv[U][VB / 4], vv[U][VB / 4], ek[U], ev[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if ((unsigned)p[u] >= (unsigned)a.L.npag) {
-                if (vis[u] && c == 0) reporta(E_ARG, a.kid, (long long)q.b * a.L.P + (j[u] >> a.L.lgpag), p[u], j[u]);
-                p[u] = 0;
-                vis[u] = false;
-            }
+            const bool fora = (unsigned)p[u] >= (unsigned)a.L.npag;
+            ruim = vis[u] && fora ? j[u] : ruim;
+            vis[u] = vis[u] && !fora;
+            p[u] = fora ? 0 : p[u];
             const long long vaga = (long long)hk * pag + (j[u] & (pag - 1));
             const int8_t *km = a.cm + p[u] * a.pag_m + vaga * HD + c * VB, *ke = a.cE + p[u] * a.pag_e + vaga * G + g;
 #pragma unroll
@@ -212,7 +221,7 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
             t[u] = vis[u] ? t[u] : -INFINITY;
             mn = fmaxf(mn, t[u]);
         }
-        const float mL = mn == -INFINITY ? 0.f : atc::vezes_log2e(mn), al = atc::fator(m, mn);
+        const float mL = mn == -INFINITY ? 0.f : atc::vezes(mn, atc::LOG2E), al = atc::fator(m, mn);
         m = mn;
         l *= al;
 #pragma unroll
@@ -226,6 +235,8 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
             for (int d = 0; d < VB; d++) o[d] += pv * (float)(int8_t)(vv[u][d / 4] >> (8 * (d % 4)));
         }
     }
+
+    atc::relata_pagina(a, q.b, ruim);
 
     // the wave's groups: a common maximum, then sums in which every step halves the values a lane still holds
     float M = m;
@@ -304,6 +315,7 @@ __global__ void __launch_bounds__(256) k_atc_junta(const float* __restrict__ ml,
     const int r = blockIdx.x, col = (blockIdx.y * 256 + threadIdx.x) * 4;
     if (col >= C) return;
     const long long part = ((long long)r * (C / hd) + col / hd) * S;
+    if (ml[2 * part] == INFINITY) return;                             // written by its one split
     float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < S; s++) M = fmaxf(M, ml[2 * (part + s)]);
     for (int s = 0; s < S; s++) {
@@ -336,6 +348,16 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef int i4_t __attribute__((ext_vector_type(4)));
+// The wait states an MFMA's result needs before another unit reads it, for results that more than one path reaches (the
+// compiler counts them along one)
+template <int N>
+__device__ __forceinline__ void pronto(f4_t (&x)[N]) {
+    static_assert(N == 1 || N == 2 || N == 4 || N == 8, "");
+    if constexpr (N == 1) asm volatile("s_nop 7" : "+v"(x[0]));
+    else if constexpr (N == 2) asm volatile("s_nop 7" : "+v"(x[0]), "+v"(x[1]));
+    else if constexpr (N == 4) asm volatile("s_nop 7" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+    else asm volatile("s_nop 7" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
+}
 constexpr int OCULTA = -2;                       // in place of a page: a key that no row of the workgroup sees
 
 // A row without visible tokens: its outputs (or the marks of its split) for the query heads of kv head hk, by the whole
@@ -343,7 +365,7 @@ constexpr int OCULTA = -2;                       // in place of a page: a key th
 template <int HD>
 __device__ __forceinline__ void vazia(const Args& a, long long r, int hk) {
     const int Gq = a.H / a.Hk, C = a.H * HD;
-    for (int x = threadIdx.x; x < Gq * HD; x += 256) {
+    for (int x = threadIdx.x; x < Gq * HD; x += blockDim.x) {
         const int h = hk * Gq + x / HD;
         const long long o = r * C + h * HD + x % HD;
         if (a.ml) {
@@ -381,6 +403,7 @@ __device__ __forceinline__ bool linhas_de(const Args& a, int b, int tile, int po
 template <int TK>
 struct Tiles {
     int lo, ns, nst, prim, t0, t1;
+    bool uma;                                    // one split takes them all
     __device__ __forceinline__ Tiles(const Args& a, int i_lo, int i_hi) {
         lo = a.janela > 0 ? max(0, i_lo + 1 - a.janela) : 0;
         ns = min(a.sumid, lo);
@@ -389,20 +412,20 @@ struct Tiles {
         const int T = nst + i_hi / TK - prim + 1;
         t0 = min((long long)blockIdx.z * a.fatia, (long long)T);
         t1 = min(t0 + a.fatia, T);
+        uma = T <= a.fatia;
     }
     __device__ __forceinline__ int j0(int t) const { return TK * (t < nst ? t : t - nst + prim); }
 };
-// the page of key j where some row sees it, else OCULTA (also a page outside the cache, which is reported)
+// the page of key j where some row sees it, else OCULTA; of a page outside the cache the key is kept in `ruim`, to be
+// reported once the loop is over (a call inside it would cost the loop its scalar registers)
 template <class T>
-__device__ __forceinline__ int pagina(const Args& a, const T& tl, int b, int t, int j, int i_hi, bool relata) {
+__device__ __forceinline__ int pagina(const Args& a, const T& tl, int b, int t, int j, int i_hi, int& ruim) {
     const bool vis = t < tl.t1 && j <= i_hi && (j >= tl.lo || j < tl.ns);
     const int p = a.L.tab[(long long)b * a.L.P + (vis ? j >> a.L.lgpag : 0)];
-    if (!vis) return OCULTA;
-    if ((unsigned)p < (unsigned)a.L.npag) return p;
-    if (relata) reporta(E_ARG, a.kid, (long long)b * a.L.P + (j >> a.L.lgpag), p, j);
-    return OCULTA;
+    const bool fora = (unsigned)p >= (unsigned)a.L.npag;
+    ruim = vis && fora ? j : ruim;
+    return vis && !fora ? p : OCULTA;
 }
-
 // the bytes 32 k + 8 c .. + 7 of a head row: a lane's share of the k-th MFMA (zeros past the head's width)
 template <int HD>
 __device__ __forceinline__ long fragmento(const int8_t* linha, int k, int c) {
@@ -443,7 +466,7 @@ struct Linha {
             x[2] += (float)p[2] * f[g].z * fq[g]; x[3] += (float)p[3] * f[g].w * fq[g];
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) s[k] = x[k] - incl * (float)(i - j - k);
+        for (int k = 0; k < 4; k++) s[k] = __builtin_fmaf(-incl, (float)(i - j) - (float)k, x[k]);   // distances below 2^24 are exact
     }
     __device__ __forceinline__ bool ve(const Args& a, int j) const { return j <= i && (a.janela <= 0 || j > i - a.janela || j < a.sumid); }
 };
@@ -460,26 +483,26 @@ struct Corrente {
     }
     // weights of a row's scores s (4 keys of every 16 in a lane) as three bf16 pieces, 24 bits, exactly
     template <int N>
-    __device__ __forceinline__ void pesos(const float (&s)[N], i4_t (&p)[3][N / 8]) {
+    __device__ __forceinline__ void pesos(const float (&s)[N], i4_t (&p)[3][N / 8], float K = LOG2E) {
         float mx = s[0];
 #pragma unroll
         for (int k = 1; k < N; k++) mx = fmaxf(mx, s[k]);
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        if (__any(mx > m + 5.f)) {
-            const float mn = fmaxf(m, mx), al = fator(m, mn);
+        if (__any(mx > m + 7.2f / K)) {                               // 2^7.2: 5 nats
+            const float mn = fmaxf(m, mx), al = fator(m, mn, K);
             m = mn;
             l *= al;
 #pragma unroll
             for (int d = 0; d < DT; d++) o[d] *= al;
         }
-        const float mL = m == -INFINITY ? 0.f : vezes_log2e(m);
+        const float mL = m == -INFINITY ? 0.f : vezes(m, K);
 #pragma unroll
         for (int k = 0; k < N; k += 2) {
             int y[3][2];
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                const float e = peso(s[k + x], mL);
+                const float e = peso(s[k + x], mL, K);
                 l += e;
                 y[0][x] = __float_as_int(e);
                 const float e1 = e - __int_as_float(y[0][x] & 0xffff0000);
@@ -504,17 +527,22 @@ struct Corrente {
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(b8_t, p1), o[d], 0, 0, 0);
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(b8_t, p2), o[d], 0, 0, 0);
         }
+        pronto(o);
     }
     __device__ __forceinline__ void soma_l() {
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
     }
-    // the row's partial result, or its output
+    // the row's output, or its partial result. `uma`: this split is the row's only one; where blocks lie in a head the output is
+    // then written here, and an infinite maximum tells the join so.
     template <int GS>
-    __device__ __forceinline__ void grava(const Args& a, long long r, int h, int c) {
+    __device__ __forceinline__ void grava(const Args& a, long long r, int h, int c, bool uma) {
         const int C = a.H * HD;
-        if (a.ml) {
-            const long long part = (r * a.H + h) * a.S + blockIdx.z;
+        const long long part = (r * a.H + h) * a.S + blockIdx.z;
+        if (a.ml && uma && a.inteira) {
+            if (blockIdx.z > 0) return;
+            if (c == 0) a.ml[2 * part] = INFINITY;
+        } else if (a.ml) {
             if (c == 0) { a.ml[2 * part] = m; a.ml[2 * part + 1] = l; }
             if (HD >= 16 || c == 0)
 #pragma unroll
@@ -578,72 +606,101 @@ __device__ __forceinline__ int4 le_vb(const int8_t* p) {
 }
 }  // namespace atc
 
-// Several rows that share keys and values (new tokens of a sequence, query heads of a group): 64 of them per workgroup, 16 a
-// wave, on matrix cores; the workgroup walks its keys in tiles of 64. Row rho of a (sequence, kv head) is token rho / Gq,
+// Many rows that share keys and values (new tokens of a sequence, query heads of a group): 16 a wave, 16 NW per workgroup, on
+// matrix cores; the workgroup walks its keys in tiles of 64. Row rho of a (sequence, kv head) is token rho / Gq,
 // head rho % Gq of the group.
-//   S^T = K Q^T by i8 MFMA, exact in int32, one accumulator per exponent group: a lane holds one row (lane % 16) and 4 keys of
-//   each 16, so maxima and sums are in-lane but for two exchanges, and P^T is the next product's operand as it stands.
-//   O^T = V^T P^T by bf16 MFMA: V's values m 2^E are exact in bf16 (8 bits), P is three bf16 pieces, exact too (one piece
-//   would leave 2^-8 of every weight, two 2^-16). V^T comes from row-major LDS by transposing reads.
+//   S^T = K Q^T by bf16 MFMA on the values m 2^E themselves, exact in bf16 (8 bits), sums in fp32: a lane holds one row (lane %
+//   16) and 4 keys of each 16, so maxima and sums are in-lane but for two exchanges, and P^T is the next product's
+//   operand as it stands. (i8 MFMA, exact, costs a conversion and two products per score and exponent group: 281 us for
+//   the prompts below.)
+//   O^T = V^T P^T by bf16 MFMA: P is three bf16 pieces, exact (one piece would leave 2^-8 of every weight, two 2^-16). V^T
+//   comes from row-major LDS by transposing reads.
 // Keys and values are staged once per workgroup, two tiles in LDS: the next tile's loads are in flight while this one is
 // computed, its page numbers one tile earlier still. Slots no row sees are staged as zeros, whatever they hold. The running maximum is
 // raised (and O rescaled) only where a tile exceeds it by 5 nats: weights are then at most e^5, which costs fp32 no precision.
-template <int HD, int GS>
-__global__ void __launch_bounds__(256) k_atc_mf(atc::Args a, int por_seq) {
+template <int HD, int GS, int NW>
+__global__ void __launch_bounds__(64 * NW) k_atc_mf(atc::Args a, int por_seq) {
     using namespace atc;
-    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 64, NM = Linha<HD, GS>::NM;
-    constexpr int KS = HD < 16 ? 4 : HD + 8, VS = 16 * Corrente<HD>::DT + 8;                  // LDS rows, in values
-    constexpr int NT = 2 * TK * LPK, IT = (NT + 255) / 256, NK = IT == 4 ? 2 : 1;             // staging: tasks, per thread; keys of a thread
-    __shared__ __align__(16) int8_t sk[2][TK * KS];
-    __shared__ __align__(16) __bf16 sv[2][TK * VS];
-    __shared__ __align__(16) float sf[2][G * TK];
+    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 64, NM = HD < 32 ? 1 : HD / 32, RW = 16 * NW;
+    constexpr int VS = 16 * Corrente<HD>::DT + 8;                     // LDS rows, in values; keys and values alike
+    constexpr int NT = TK * LPK, IT = (NT + 64 * NW - 1) / (64 * NW); // staging: chunks of a tile's keys (and of its values), per thread
+    __shared__ __align__(16) __bf16 sk[2][TK * VS], sv[2][TK * VS];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk;
-    const int b = blockIdx.x / por_seq, tile = por_seq - 1 - blockIdx.x % por_seq;            // a sequence's last rows, the longest, first
+    const int b = blockIdx.x % (a.L.B + 1), tile = por_seq - 1 - blockIdx.x / (a.L.B + 1);    // the last rows, with the most keys, first
     int r0, n, comp;
-    if (!linhas_de<HD>(a, b, tile, por_seq, 64, hk, r0, n, comp)) return;
-    const int linhas = n * Gq, rho0 = tile * 64, i_lo = comp - n + rho0 / Gq, i_hi = comp - n + min(rho0 + 63, linhas - 1) / Gq;
+    if (!linhas_de<HD>(a, b, tile, por_seq, RW, hk, r0, n, comp)) return;
+    const int linhas = n * Gq, rho0 = tile * RW, i_lo = comp - n + rho0 / Gq, i_hi = comp - n + min(rho0 + RW - 1, linhas - 1) / Gq;
     const Tiles<TK> tl(a, i_lo, i_hi);
     const int rho = rho0 + 16 * w + lr, w_hi = comp - n + min(rho0 + 16 * w + 15, linhas - 1) / Gq;   // w_hi: the wave's last position
     const bool tem = rho0 + 16 * w < linhas;
-    const Linha<HD, GS> q(a, r0, n, comp, hk, min(rho, linhas - 1), c);
+
+    // this lane's query row as MFMA operands: m 2^E in bf16, exact
+    const int rc = min(rho, linhas - 1), h = hk * Gq + rc % Gq, i = comp - n + rc / Gq, ld = (a.H + 2 * a.Hk) * HD;
+    const long long r = r0 + rc / Gq;
+    const float raiz = __builtin_sqrtf((float)HD), K = LOG2E / raiz, incl = a.incl ? a.incl[h] * raiz : 0.f;
+    b8_t q[NM];
+#pragma unroll
+    for (int k = 0; k < NM; k++) {
+        const long x = fragmento<HD>(a.qm + r * ld + h * HD, k, c);
+        const int col = h * HD + (HD >= 32 ? 32 * k + 8 * c : 0);
+        const float e = __builtin_ldexpf(1.f, a.qE[r * (ld >> a.lgblk) + (col >> a.lgblk)]);
+#pragma unroll
+        for (int z = 0; z < 8; z++) q[k][z] = (__bf16)(e * (float)(int8_t)(x >> (8 * z)));
+    }
 
     const int pag = 1 << a.L.lgpag;
-    int pg[NK];
-    int4 dm[IT];
-    int de[IT];
-    auto chave = [&](int k) { return (int)((threadIdx.x / LPK + 32 * k) % TK); };
+    const long long dvm = (long long)a.Hk * pag * HD, dve = (long long)a.Hk * pag * G;        // from a key to its value
+    int pg[IT], de[2][IT], ruim = -1;
+    int4 dm[2][IT];
+    auto chave = [&](int x) { return (int)(threadIdx.x + 64 * NW * x) / LPK; };
+    // A tile lies in one page where pages hold 64 slots or more: one scalar table read, and a thread's chunk is at a fixed offset
+    // of the tile. Smaller pages are looked up key by key.
+    const bool uma = pag >= TK;
     auto le_paginas = [&](int t) {
+        if (uma) {
+            const int j0 = tl.j0(t), j = min(max(j0, j0 >= tl.prim * TK ? tl.lo : 0), i_hi);  // a key of the tile that some row sees
+            pg[0] = t < tl.t1 ? __builtin_amdgcn_readfirstlane(a.L.tab[(long long)b * a.L.P + (j >> a.L.lgpag)]) : OCULTA;
+            if (t < tl.t1 && (unsigned)pg[0] >= (unsigned)a.L.npag) { ruim = j; pg[0] = OCULTA; }
+            return;
+        }
 #pragma unroll
-        for (int k = 0; k < NK; k++) pg[k] = pagina(a, tl, b, t, tl.j0(t) + chave(k), i_hi, hk == 0 && threadIdx.x % LPK == 0);
+        for (int x = 0; x < IT; x++) pg[x] = (int)threadIdx.x + 64 * NW * x < NT ? pagina(a, tl, b, t, tl.j0(t) + chave(x), i_hi, ruim) : OCULTA;
     };
-    // task: a chunk of VB bytes of a key (first TK LPK tasks) or a value, and its exponent
     auto le_dados = [&](int t) {
+        const int j0 = tl.j0(t), cc = threadIdx.x % LPK;
+        const long long base = (long long)hk * pag + (j0 & (pag - 1));
+        const int p0 = __builtin_amdgcn_readfirstlane(pg[0]);
+        const int8_t *m0 = a.cm + p0 * a.pag_m + base * HD, *e0 = a.cE + p0 * a.pag_e + base * G;
 #pragma unroll
         for (int x = 0; x < IT; x++) {
-            const int tarefa = threadIdx.x + 256 * x, k = NK == 2 ? x & 1 : 0, kv = tarefa / (TK * LPK), cc = tarefa % LPK;
-            dm[x] = make_int4(0, 0, 0, 0);
-            de[x] = -127;
-            if (tarefa < NT && pg[k] != OCULTA) {
-                const long long vaga = ((long long)kv * a.Hk + hk) * pag + ((tl.j0(t) + chave(k)) & (pag - 1));
-                dm[x] = le_vb<VB>(a.cm + pg[k] * a.pag_m + vaga * HD + cc * VB);
-                de[x] = a.cE[pg[k] * a.pag_e + vaga * G + cc * VB / GS];
+            dm[0][x] = dm[1][x] = make_int4(0, 0, 0, 0);
+            de[0][x] = de[1][x] = -127;
+            const int key = chave(x), j = j0 + key;
+            if (uma) {
+                if (p0 != OCULTA && (int)threadIdx.x + 64 * NW * x < NT && j <= i_hi && (j >= tl.lo || j < tl.ns)) {
+                    const int8_t *p = m0 + (threadIdx.x + 64 * NW * x) * VB, *e = e0 + key * G + cc * VB / GS;
+                    dm[0][x] = le_vb<VB>(p);
+                    dm[1][x] = le_vb<VB>(p + dvm);
+                    de[0][x] = e[0];
+                    de[1][x] = e[dve];
+                }
+            } else if (pg[x] != OCULTA) {
+                const long long vaga = (long long)hk * pag + (j & (pag - 1));
+                const int8_t *p = a.cm + pg[x] * a.pag_m + vaga * HD + cc * VB, *e = a.cE + pg[x] * a.pag_e + vaga * G + cc * VB / GS;
+                dm[0][x] = le_vb<VB>(p);
+                dm[1][x] = le_vb<VB>(p + dvm);
+                de[0][x] = e[0];
+                de[1][x] = e[dve];
             }
         }
     };
     auto guarda = [&](int buf) {
 #pragma unroll
         for (int x = 0; x < IT; x++) {
-            const int tarefa = threadIdx.x + 256 * x, k = NK == 2 ? x & 1 : 0, kv = tarefa / (TK * LPK), cc = tarefa % LPK, key = chave(k);
-            if (tarefa >= NT) continue;
-            const float e = __builtin_ldexpf(1.f, de[x]);
-            if (kv == 0) {
-                int8_t* p = &sk[buf][key * KS + cc * VB];
-                if constexpr (VB == 16) {
-                    reinterpret_cast<int2*>(p)[0] = make_int2(dm[x].x, dm[x].y);
-                    reinterpret_cast<int2*>(p)[1] = make_int2(dm[x].z, dm[x].w);
-                } else *reinterpret_cast<int*>(p) = dm[x].x;
-                if (cc * VB % GS == 0) sf[buf][cc * VB / GS * TK + key] = e;
-            } else valor_lds<VB>(&sv[buf][key * VS + cc * VB], dm[x], e);
+            if ((int)threadIdx.x + 64 * NW * x >= NT) continue;
+            const int o = chave(x) * VS + threadIdx.x % LPK * VB;
+            valor_lds<VB>(&sk[buf][o], dm[0][x], __builtin_ldexpf(1.f, de[0][x]));
+            valor_lds<VB>(&sv[buf][o], dm[1][x], __builtin_ldexpf(1.f, de[1][x]));
         }
     };
 
@@ -660,32 +717,44 @@ __global__ void __launch_bounds__(256) k_atc_mf(atc::Args a, int por_seq) {
         if (t + 1 < tl.t1) { le_dados(t + 1); le_paginas(t + 2); }
         if (tem && j0 <= w_hi) {
             float s[16];
+            f4_t x[4];
+            const float bias = -incl * (float)(i - j0 - 4 * c);       // the product starts from the bias of each key
 #pragma unroll
             for (int kt = 0; kt < 4; kt++) {
-                long kf[NM];
-                float4 f[G];
 #pragma unroll
-                for (int k = 0; k < NM; k++) kf[k] = fragmento<HD>(&sk[buf][(16 * kt + lr) * KS], k, c);
+                for (int k = 0; k < 4; k++) x[kt][k] = __builtin_fmaf(incl, (float)(16 * kt + k), bias);
 #pragma unroll
-                for (int g = 0; g < G; g++) f[g] = *reinterpret_cast<const float4*>(&sf[buf][g * TK + 16 * kt + 4 * c]);
-                q.notas(kf, f, j0 + 16 * kt + 4 * c, s + 4 * kt);
+                for (int k = 0; k < NM; k++) {
+                    b8_t kf = b8_t{};
+                    if (HD >= 32 || c < 2) kf = *reinterpret_cast<const b8_t*>(&sk[buf][(16 * kt + lr) * VS + 32 * k + 8 * c]);
+                    x[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[k], x[kt], 0, 0, 0);
+                }
             }
+            pronto(x);
+#pragma unroll
+            for (int k = 0; k < 16; k++) s[k] = x[k / 4][k % 4];
             // every key of the tile visible to every row of the workgroup: nothing to mask
             if (j0 + TK - 1 > i_lo || (a.janela > 0 && j0 <= i_hi - a.janela && j0 + TK > a.sumid)) {
+                const int janela = a.janela > 0 ? a.janela : 0x7fffffff;
 #pragma unroll
-                for (int k = 0; k < 16; k++) s[k] = q.ve(a, j0 + 16 * (k / 4) + 4 * c + k % 4) ? s[k] : -INFINITY;
+                for (int k = 0; k < 16; k++) {
+                    const int j = j0 + 4 * c + 16 * (k / 4) + k % 4;
+                    s[k] = j <= i && (i - j < janela || j < a.sumid) ? s[k] : -INFINITY;
+                }
             }
             i4_t p[3][2];
-            y.pesos(s, p);
+            y.pesos(s, p, K);
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) y.template soma_v<VS>(&sv[buf][32 * kk * VS], p[0][kk], p[1][kk], p[2][kk], lr, c);
         }
         if (t + 1 < tl.t1) guarda(buf ^ 1);
         __syncthreads();
     }
+    if (hk == 0) relata_pagina(a, b, ruim);
     if (rho >= linhas) return;
     y.soma_l();
-    y.template grava<GS>(a, q.r, q.h, c);
+    y.m *= 1.f / raiz;                                                // in nats, as the join takes it
+    y.template grava<GS>(a, r, h, c, tl.uma);
 }
 
 // Up to 16 rows that share keys and values (a new token's query heads of a group, a few new tokens): the same products, but the
@@ -710,17 +779,17 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
     const Linha<HD, GS> q(a, r0, n, comp, hk, min(lr, linhas - 1), c);
 
     // a lane's keys: lr and 16 + lr of the tile for the products; lane / LPK, then 64 / LPK further on, for the values
-    int pk[2], pv[IT], ke[2];
+    int pk[2], pv[IT], ke[2], ruim = -1;
     long kf[2][NM];
     int4 dv[IT];
     int ve[IT];
     auto le_paginas = [&](int t) {
 #pragma unroll
-        for (int k = 0; k < 2; k++) pk[k] = pagina(a, tl, b, t, tl.j0(t) + 16 * k + lr, i_hi, hk == 0 && c == 0);
+        for (int k = 0; k < 2; k++) pk[k] = pagina(a, tl, b, t, tl.j0(t) + 16 * k + lr, i_hi, ruim);
 #pragma unroll
         for (int x = 0; x < IT; x++) {
             const int key = lane / LPK + 64 / LPK * x;
-            pv[x] = key < TK ? pagina(a, tl, b, t, tl.j0(t) + key, i_hi, false) : OCULTA;
+            pv[x] = key < TK ? pagina(a, tl, b, t, tl.j0(t) + key, i_hi, ruim) : OCULTA;
         }
     };
     auto le_dados = [&](int t) {
@@ -790,6 +859,7 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
         y.template soma_v<VS>(sv, p[0][0], p[1][0], p[2][0], lr, c);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+    relata_pagina(a, b, ruim);
     // the four waves' results: a common maximum, then sums
     y.soma_l();
     if (c == 0) { sm[w][lr] = y.m; sl[w][lr] = y.l; }
@@ -814,7 +884,7 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
         for (int k = 0; k < 3; k++) y.o[d] += so[(k * DT + d) * 64 + lane];
     y.m = M;
     y.l = L;
-    y.template grava<GS>(a, q.r, q.h, c);
+    y.template grava<GS>(a, q.r, q.h, c, tl.uma);
 }
 
 // ---------------------------------------------------------------------------------------------- values
