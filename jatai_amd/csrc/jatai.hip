@@ -1046,34 +1046,42 @@ int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, in
 }
 
 // How a call runs, by the rows that share a kv head's keys at most: one (k_atc_um, a row per workgroup), up to 16 (k_atc_gr) or
-// more (k_atc_mf, 16 ATC_NW rows a workgroup, por_seq workgroups a sequence). S splits of the visible tokens, `fatia` tokens (um) or
+// more (k_atc_mf, 64 rows a workgroup). S splits of the visible tokens, `fatia` tokens (um) or
 // tiles of 32 (gr) or 64 (mf) tokens each: as many as fill the chip, each with at least one step of a workgroup's loop (um), two
 // tiles a wave (gr) or four tiles (mf). direto: one split, and every block of the output lies in a head, so the kernel
 // writes it and there is no join.
 enum { ATC_UM, ATC_GR, ATC_MF };
+#ifndef ATC_UMAX
+#define ATC_UMAX 1
+#endif
+#ifndef ATC_ALVO
+#define ATC_ALVO 2048
+#endif
 #ifndef ATC_FATIA
 #define ATC_FATIA 24
 #endif
-constexpr int ATC_NW = 4;                                            // waves of a k_atc_mf workgroup
-struct PlanoAtc { int tipo; bool direto; int por_seq, S, fatia; };
+struct PlanoAtc { int tipo; bool direto; unsigned tiles; int S, fatia; };
 static PlanoAtc atc_plano(long long M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo) {
     PlanoAtc p;
     const long long linhas = (long long)novos * (H / Hk);
-    p.tipo = linhas > 16 ? ATC_MF : linhas > 1 ? ATC_GR : ATC_UM;
-    p.por_seq = p.tipo == ATC_MF ? (int)((linhas + 16 * ATC_NW - 1) / (16 * ATC_NW)) : 1;
-    long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto), passo, wgs, alvo = 2048;
+        p.tipo = linhas > 16 ? ATC_MF : linhas > ATC_UMAX ? ATC_GR : ATC_UM;
+    const bool mf = p.tipo == ATC_MF;
+    const long long por_wg = 64;
+    // every sequence's tiles (its last one may be cut short), and one workgroup at least for the rows of no sequence
+    p.tiles = (unsigned)std::min((M * (H / Hk) + por_wg - 1) / por_wg + B + 1, 0x7fffffffLL);
+    long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto), passo, wgs, alvo = ATC_ALVO;
     if (p.tipo == ATC_UM) {
         passo = hd <= 16 ? 1024 : 16384 / hd;
         wgs = M * H;
     } else {                                                         // in tiles: a window's may begin and end inside one, the first tokens' too
-        const long long tk = p.tipo == ATC_MF ? 64 : 32, nt = (teto + tk - 1) / tk;
-        nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, 16LL * ATC_NW) + tk - 2) / tk + 1 + (sumid + tk - 1) / tk) : nt);
-        passo = p.tipo == ATC_MF ? 4 : 8;
-        if (p.tipo == ATC_MF) alvo = 1024;
-        wgs = (long long)B * p.por_seq * Hk;
+        const long long tk = mf ? 64 : 32, nt = (teto + tk - 1) / tk;
+        nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, por_wg) + tk - 2) / tk + 1 + (sumid + tk - 1) / tk) : nt);
+        passo = mf ? 4 : 8;
+        if (mf) alvo = 1024;
+        wgs = (mf ? (M * (H / Hk) + por_wg - 1) / por_wg : (long long)B) * Hk;
     }
     long long s = std::min(std::max(alvo / std::max(wgs, 1LL), 1LL), (nv + passo - 1) / passo);
-    if (p.tipo == ATC_MF) s = std::max(s, (nv + ATC_FATIA - 1) / ATC_FATIA);
+    if (mf) s = std::max(s, (nv + ATC_FATIA - 1) / ATC_FATIA);
     p.fatia = (int)(((nv + s - 1) / s + passo - 1) / passo * passo);
     p.S = (int)((nv + p.fatia - 1) / p.fatia);
     p.direto = p.tipo != ATC_UM && p.S == 1 && (tipo != 0 || hd >= g_blk);
@@ -1093,14 +1101,14 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
     if (janela < 0 || sumid < 0 || tipo < 0 || tipo > 2 || (tipo == 0 && (!outE || H * hd % g_blk))) return (int)hipErrorInvalidValue;
     const PlanoAtc p = atc_plano(M, B, H, Hk, hd, novos, teto, janela, sumid, tipo);
     if (!p.direto && (!ws || ws_bytes < jt_atencao_cache_ws_bytes(M, B, H, Hk, hd, novos, teto, janela, sumid, tipo))) return (int)hipErrorInvalidValue;
-    if (p.S > 65535 || (long long)(B + 1) * p.por_seq > 0x7fffffff) return (int)hipErrorInvalidValue;
+    if (p.S > 65535 || p.tiles == 0x7fffffff || B == 0x7fffffff) return (int)hipErrorInvalidValue;
     const long long camada_m = 2LL * Hk * pag * hd, camada_e = 2LL * Hk * pag * grupos(hd), partes = (long long)M * H * p.S;
     float *ml = p.direto ? nullptr : (float*)ws, *po = p.direto ? nullptr : ml + (2 * partes + 3) / 4 * 4;
     const atc::Args a{(const int8_t*)qm, (const int8_t*)qE, (const int8_t*)cm + camada * camada_m, (const int8_t*)cE + camada * camada_e,
                       (const float*)incl, ml, po, out, (int8_t*)outE, camadas * camada_m, camadas * camada_e,
                       atc::Lote{(const int*)tab, (const int*)comp, (const int*)ini, B, P, M, ilog2(pag), npag, novos, teto},
                       tipo != 0 || hd >= g_blk, H, Hk, ilog2(g_blk), janela, sumid, p.S, p.fatia, tipo, kid};
-#define F(HD, GS) (p.tipo == ATC_MF ? k_atc_mf<HD, GS, ATC_NW><<<dim3((B + 1) * p.por_seq, Hk, p.S), 64 * ATC_NW, 0, g_stream>>>(a, p.por_seq) \
+#define F(HD, GS) (p.tipo == ATC_MF ? k_atc_mf<HD, GS><<<dim3(p.tiles, Hk, p.S), 256, 0, g_stream>>>(a) \
                    : p.tipo == ATC_GR ? k_atc_gr<HD, GS><<<dim3(B + 1, Hk, p.S), 256, 0, g_stream>>>(a) \
                                       : k_atc_um<HD, GS><<<dim3(M, H, p.S), 256, 0, g_stream>>>(a))
     POR_CABECA(F)
@@ -1108,8 +1116,10 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
     int rc = fim();
     if (rc || p.direto) return rc;
     const int C = H * hd;
-    const dim3 grade(M, (C + 1023) / 1024);
-#define J(BL, T) (k_atc_junta<BL, T><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid))
+    const dim3 grade(M, (C + 127) / 128);
+#define J(BL, T) (p.S <= 8 ? k_atc_junta<BL, T, 2><<<grade, 64, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)       \
+                  : p.S <= 32 ? k_atc_junta<BL, T, 8><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)   \
+                              : k_atc_junta<BL, T, 32><<<grade, 1024, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid))
     if (tipo == 1) J(32, 1);
     else if (tipo == 2) J(32, 2);
     else if (g_blk == 32) J(32, 0);

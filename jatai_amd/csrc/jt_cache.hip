@@ -308,22 +308,57 @@ __device__ __forceinline__ int quant_f32(const float (&v)[NV], int8_t (&q)[NV], 
 }
 
 // Joins the splits of a row and head, o = sum exp(m_s - m) o_s / sum exp(m_s - m) l_s (zeros for a row without visible
-// tokens), 4 columns a thread, and writes the row as a block tensor (TIPO 0), bfloat16 (1) or fp32 (2).
-template <int BLK, int TIPO>
-__global__ void __launch_bounds__(256) k_atc_junta(const float* __restrict__ ml, const float* __restrict__ po, void* __restrict__ out,
-                                                   int8_t* __restrict__ oE, int C, int hd, int S, int kid) {
-    const int r = blockIdx.x, col = (blockIdx.y * 256 + threadIdx.x) * 4;
-    if (col >= C) return;
-    const long long part = ((long long)r * (C / hd) + col / hd) * S;
-    if (ml[2 * part] == INFINITY) return;                             // written by its one split
+// tokens), and writes the row as a block tensor (TIPO 0), bfloat16 (1) or fp32 (2). A workgroup takes 128 columns of a row, 4 a
+// thread, and shares the splits out among its NG groups of 32 threads, four of them in flight at a time: one
+// thread walking 64 splits one by one waited for each (30 us of a call of 131).
+template <int BLK, int TIPO, int NG>
+__global__ void __launch_bounds__(32 * NG) k_atc_junta(const float* __restrict__ ml, const float* __restrict__ po, void* __restrict__ out,
+                                                    int8_t* __restrict__ oE, int C, int hd, int S, int kid) {
+    const int r = blockIdx.x, ct = threadIdx.x & 31, g = threadIdx.x >> 5, col = blockIdx.y * 128 + 4 * ct, cc = min(col, C - 4);
+    const long long part = ((long long)r * (C / hd) + cc / hd) * S;
+    const bool escrita = ml[2 * part] == INFINITY || col >= C;        // by its one split
+    if (__all(escrita)) return;                                       // every wave has the same columns
     float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < S; s++) M = fmaxf(M, ml[2 * (part + s)]);
-    for (int s = 0; s < S; s++) {
-        const float m = ml[2 * (part + s)];
-        if (m == -INFINITY) continue;
-        const float f = atc::fator(m, M);
-        L += f * ml[2 * (part + s) + 1];
-        const float4 x = *reinterpret_cast<const float4*>(po + (part + s) * hd + col % hd);
+    for (int s0 = g; s0 < S; s0 += 4 * NG) {
+        float2 x[4];
+        float4 y[4];
+        float mn = M;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int s = s0 + k * NG;
+            x[k] = *reinterpret_cast<const float2*>(ml + 2 * (part + min(s, S - 1)));
+            y[k] = *reinterpret_cast<const float4*>(po + (part + min(s, S - 1)) * hd + cc % hd);
+            x[k].x = s < S && x[k].x != INFINITY ? x[k].x : -INFINITY;
+            mn = fmaxf(mn, x[k].x);
+        }
+        const float al = atc::fator(M, mn);
+        M = mn;
+        L *= al;
+#pragma unroll
+        for (int d = 0; d < 4; d++) v[d] *= al;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {                                 // a split without tokens has left its outputs unwritten
+            const float f = atc::fator(x[k].x, M);
+            const bool tem = f > 0.f;
+            L += tem ? f * x[k].y : 0.f;
+            v[0] += tem ? f * y[k].x : 0.f; v[1] += tem ? f * y[k].y : 0.f;
+            v[2] += tem ? f * y[k].z : 0.f; v[3] += tem ? f * y[k].w : 0.f;
+        }
+    }
+    __shared__ float sm[NG][32], sl[NG][32];
+    __shared__ float4 sv[NG][32];
+    sm[g][ct] = M;
+    sl[g][ct] = L;
+    sv[g][ct] = make_float4(v[0], v[1], v[2], v[3]);
+    __syncthreads();
+    if (g > 0 || escrita) return;
+    float MM = M;
+    for (int k = 1; k < NG; k++) MM = fmaxf(MM, sm[k][ct]);
+    L = v[0] = v[1] = v[2] = v[3] = 0.f;
+    for (int k = 0; k < NG; k++) {
+        const float f = atc::fator(sm[k][ct], MM);
+        const float4 x = sv[k][ct];
+        L += f * sl[k][ct];
         v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -358,7 +393,6 @@ __device__ __forceinline__ void pronto(f4_t (&x)[N]) {
     else if constexpr (N == 4) asm volatile("s_nop 7" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
     else asm volatile("s_nop 7" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
 }
-constexpr int OCULTA = -2;                       // in place of a page: a key that no row of the workgroup sees
 
 // A row without visible tokens: its outputs (or the marks of its split) for the query heads of kv head hk, by the whole
 // workgroup
@@ -378,24 +412,48 @@ __device__ __forceinline__ void vazia(const Args& a, long long r, int hk) {
     }
 }
 
-// The rows that workgroup (sequence b, tile of `por_wg` rows) has; false: none (rows of no sequence and of a malformed one are
-// zeroed here). b = B: the rows of no sequence, shared out among the tiles.
+// Workgroup x as a tile of `por_wg` rows of a sequence: the sequences' tiles are numbered one after another, each sequence's last
+// rows, which see the most keys, first. Every wave scans 64 sequences at a time. b = B past the last of the `total` tiles.
+__device__ __forceinline__ void tile_de(const Args& a, int x, int por_wg, int& b, int& tile, int& total) {
+    const int lane = threadIdx.x & 63, Gq = a.H / a.Hk;
+    b = a.L.B;
+    total = 0;
+    for (int k = 0; k < a.L.B; k += 64) {
+        const int s = min(k + lane, a.L.B - 1), n = a.L.ini ? a.L.ini[s + 1] - a.L.ini[s] : min(a.L.comp[s], 1);
+        const int tiles = k + lane < a.L.B ? (int)(((long long)min(max(n, 0), a.L.M) * Gq + por_wg - 1) / por_wg) : 0;
+        int ate = tiles;                                              // of this sequence and those before it
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int y = __shfl_up(ate, d);
+            ate += lane >= d ? y : 0;
+        }
+        if (b == a.L.B && x < total + __shfl(ate, 63)) {
+            const int q = __popcll(__ballot(total + ate <= x));
+            b = k + q;
+            tile = total + __shfl(ate, q) - 1 - x;
+        }
+        total += __shfl(ate, 63);
+    }
+}
+
+// Rows r0 .. r0 + n - 1 of sequence b, comp tokens long; false (its rows, if any, zeroed) where it is malformed or has none. b = B:
+// the rows of no sequence, every `passo`-th from `parte` on.
 template <int HD>
-__device__ __forceinline__ bool linhas_de(const Args& a, int b, int tile, int por_seq, int por_wg, int hk, int& r0, int& n, int& comp) {
+__device__ __forceinline__ bool linhas_de(const Args& a, int b, bool primeiro, int parte, int passo, int hk, int& r0, int& n, int& comp) {
     if (b == a.L.B) {
         const int ini = a.L.ini ? a.L.ini[0] : 0, fim = a.L.ini ? a.L.ini[a.L.B] : a.L.B;
-        for (long long x = tile; x < min(ini, a.L.M); x += por_seq) vazia<HD>(a, x, hk);
-        for (long long x = max(fim, 0) + (long long)tile; x < a.L.M; x += por_seq) vazia<HD>(a, x, hk);
+        for (long long x = parte; x < min(ini, a.L.M); x += passo) vazia<HD>(a, x, hk);
+        for (long long x = max(fim, 0) + (long long)parte; x < a.L.M; x += passo) vazia<HD>(a, x, hk);
         return false;
     }
-    if (!sequencia(a.L, b, r0, n, comp, a.kid, threadIdx.x == 0 && hk == 0 && blockIdx.z == 0 && tile == 0)) {
+    if (!sequencia(a.L, b, r0, n, comp, a.kid, primeiro && threadIdx.x == 0 && hk == 0 && blockIdx.z == 0)) {
         const long long fim = a.L.ini ? (long long)a.L.ini[b + 1] : b + 1;
-        if (tile == 0)
+        if (primeiro)
             for (long long r = max(r0, 0); r < min(fim, (long long)a.L.M); r++) vazia<HD>(a, r, hk);
         return false;
     }
-    if (!a.L.ini && n == 0 && tile == 0 && r0 < a.L.M) vazia<HD>(a, r0, hk);
-    return (long long)tile * por_wg < (long long)n * (a.H / a.Hk);
+    if (!a.L.ini && n == 0 && primeiro && r0 < a.L.M) vazia<HD>(a, r0, hk);
+    return n > 0;
 }
 
 // The tiles of TK keys that rows at positions i_lo .. i_hi see, numbered without gaps: those of the first tokens, then the
@@ -416,16 +474,20 @@ struct Tiles {
     }
     __device__ __forceinline__ int j0(int t) const { return TK * (t < nst ? t : t - nst + prim); }
 };
-// the page of key j where some row sees it, else OCULTA; of a page outside the cache the key is kept in `ruim`, to be
-// reported once the loop is over (a call inside it would cost the loop its scalar registers)
+// Whether some row sees key j of tile t
 template <class T>
-__device__ __forceinline__ int pagina(const Args& a, const T& tl, int b, int t, int j, int i_hi, int& ruim) {
-    const bool vis = t < tl.t1 && j <= i_hi && (j >= tl.lo || j < tl.ns);
-    const int p = a.L.tab[(long long)b * a.L.P + (vis ? j >> a.L.lgpag : 0)];
-    const bool fora = (unsigned)p >= (unsigned)a.L.npag;
-    ruim = vis && fora ? j : ruim;
-    return vis && !fora ? p : OCULTA;
+__device__ __forceinline__ bool visivel(const T& tl, int t, int j, int i_hi) { return (t < tl.t1) & (j <= i_hi) & ((j >= tl.lo) | (j < tl.ns)); }
+// The page-table entry of key j (of some seen key where no row sees j). It is loaded a tile before it is used: whoever looks at it
+// at once waits for every load issued before it, the tile's data among them.
+__device__ __forceinline__ int entrada(const Args& a, int b, int j, int i_hi) { return a.L.tab[(long long)b * a.L.P + (min(j, i_hi) >> a.L.lgpag)]; }
+// Entry p as a page to read from, whatever it holds (page 0 in place of one outside the cache): every load is made, without a
+// branch, and a key that no row sees counts for nothing through its scale (escala). ok: whether the page is in the cache.
+__device__ __forceinline__ int pagina(const Args& a, int p, bool& ok) {
+    ok = (unsigned)p < (unsigned)a.L.npag;
+    return ok ? p : 0;
 }
+__device__ __forceinline__ float escala(int E, bool conta) { return conta ? __builtin_ldexpf(1.f, E) : 0.f; }
+
 // the bytes 32 k + 8 c .. + 7 of a head row: a lane's share of the k-th MFMA (zeros past the head's width)
 template <int HD>
 __device__ __forceinline__ long fragmento(const int8_t* linha, int k, int c) {
@@ -468,7 +530,7 @@ struct Linha {
 #pragma unroll
         for (int k = 0; k < 4; k++) s[k] = __builtin_fmaf(-incl, (float)(i - j) - (float)k, x[k]);   // distances below 2^24 are exact
     }
-    __device__ __forceinline__ bool ve(const Args& a, int j) const { return j <= i && (a.janela <= 0 || j > i - a.janela || j < a.sumid); }
+    __device__ __forceinline__ bool ve(const Args& a, int j) const { return (j <= i) & ((a.janela <= 0) | (j > i - a.janela) | (j < a.sumid)); }
 };
 
 // The running softmax of a lane's row and the outputs it accumulates, O^T tiles of 16 dimensions (lane: row, 4 dimensions)
@@ -487,9 +549,9 @@ struct Corrente {
         float mx = s[0];
 #pragma unroll
         for (int k = 1; k < N; k++) mx = fmaxf(mx, s[k]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        if (__any(mx > m + 7.2f / K)) {                               // 2^7.2: 5 nats
+        if (__any(mx > m + 7.2f / K)) {                               // 2^7.2: 5 nats; the exchange between lanes only then
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float mn = fmaxf(m, mx), al = fator(m, mn, K);
             m = mn;
             l *= al;
@@ -512,22 +574,6 @@ struct Corrente {
 #pragma unroll
             for (int x = 0; x < 3; x++) p[x][k / 8][k % 8 / 2] = (int)__builtin_amdgcn_perm((unsigned)y[x][1], (unsigned)y[x][0], 0x07060302u);
         }
-    }
-    // O^T += V^T P^T over 32 keys, whose values are the rows of v in LDS (VS bf16 each)
-    template <int VS>
-    __device__ __forceinline__ void soma_v(const __bf16* v, const i4_t& p0, const i4_t& p1, const i4_t& p2, int lr, int c) {
-        typedef __attribute__((address_space(3))) s4_t* lds4;
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            // lane 16 c + x reads row 4 c + x / 4, columns 4 (x % 4) ..; it receives column x of the 4 rows
-            const __bf16* y = v + (4 * c + lr / 4) * VS + 16 * d + 4 * (lr % 4);
-            const s4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(y)), v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(y + 16 * VS));
-            const b8_t x = __builtin_bit_cast(b8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(b8_t, p0), o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(b8_t, p1), o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(b8_t, p2), o[d], 0, 0, 0);
-        }
-        pronto(o);
     }
     __device__ __forceinline__ void soma_l() {
         l += __shfl_xor(l, 16);
@@ -586,6 +632,29 @@ struct Corrente {
     }
 };
 
+// O^T += V^T P^T over 32 keys, whose values are the rows of v in LDS (VS bf16 each); p[.][kk]: their weights
+template <int HD, int VS, int N>
+__device__ __forceinline__ void soma_v(Corrente<HD>& y, const __bf16* v, const i4_t (&p)[3][N], int kk, int lr, int c) {
+    typedef __attribute__((address_space(3))) s4_t* lds4;
+    constexpr int DT = Corrente<HD>::DT, DB = DT < 4 ? DT : 4;        // four tiles of dimensions at a time: products in a row do not wait for one another
+#pragma unroll
+    for (int d0 = 0; d0 < DT; d0 += DB) {
+        b8_t x[DB];
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+            // lane 16 c + x reads row 4 c + x / 4, columns 4 (x % 4) ..; it receives column x of the 4 rows
+            const __bf16* z = v + (4 * c + lr / 4) * VS + 16 * (d0 + d) + 4 * (lr % 4);
+            const s4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(z)), v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(z + 16 * VS));
+            x[d] = __builtin_bit_cast(b8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+#pragma unroll
+            for (int d = 0; d < DB; d++) y.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[d], __builtin_bit_cast(b8_t, p[k][kk]), y.o[d0 + d], 0, 0, 0);
+    }
+    pronto(y.o);
+}
+
 // VB mantissas of a value and its exponent, into a row of bf16 in LDS: m 2^E is exact there. A row narrower than 16 is
 // filled up with zeros.
 template <int VB>
@@ -606,7 +675,7 @@ __device__ __forceinline__ int4 le_vb(const int8_t* p) {
 }
 }  // namespace atc
 
-// Many rows that share keys and values (new tokens of a sequence, query heads of a group): 16 a wave, 16 NW per workgroup, on
+// Many rows that share keys and values (new tokens of a sequence, query heads of a group): 16 a wave, 64 per workgroup, on
 // matrix cores; the workgroup walks its keys in tiles of 64. Row rho of a (sequence, kv head) is token rho / Gq,
 // head rho % Gq of the group.
 //   S^T = K Q^T by bf16 MFMA on the values m 2^E themselves, exact in bf16 (8 bits), sums in fp32: a lane holds one row (lane %
@@ -618,17 +687,17 @@ __device__ __forceinline__ int4 le_vb(const int8_t* p) {
 // Keys and values are staged once per workgroup, two tiles in LDS: the next tile's loads are in flight while this one is
 // computed, its page numbers one tile earlier still. Slots no row sees are staged as zeros, whatever they hold. The running maximum is
 // raised (and O rescaled) only where a tile exceeds it by 5 nats: weights are then at most e^5, which costs fp32 no precision.
-template <int HD, int GS, int NW>
-__global__ void __launch_bounds__(64 * NW) k_atc_mf(atc::Args a, int por_seq) {
+template <int HD, int GS>
+__global__ void __launch_bounds__(256) k_atc_mf(atc::Args a) {
     using namespace atc;
-    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 64, NM = HD < 32 ? 1 : HD / 32, RW = 16 * NW;
+    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 64, NM = HD < 32 ? 1 : HD / 32, RW = 64;
     constexpr int VS = 16 * Corrente<HD>::DT + 8;                     // LDS rows, in values; keys and values alike
-    constexpr int NT = TK * LPK, IT = (NT + 64 * NW - 1) / (64 * NW); // staging: chunks of a tile's keys (and of its values), per thread
+    constexpr int NT = TK * LPK, IT = (NT + 255) / 256; // staging: chunks of a tile's keys (and of its values), per thread
     __shared__ __align__(16) __bf16 sk[2][TK * VS], sv[2][TK * VS];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk;
-    const int b = blockIdx.x % (a.L.B + 1), tile = por_seq - 1 - blockIdx.x / (a.L.B + 1);    // the last rows, with the most keys, first
-    int r0, n, comp;
-    if (!linhas_de<HD>(a, b, tile, por_seq, RW, hk, r0, n, comp)) return;
+    int b, tile = 0, total, r0, n, comp;
+    tile_de(a, blockIdx.x, RW, b, tile, total);
+    if (!linhas_de<HD>(a, b, tile == 0, blockIdx.x - total, gridDim.x - total, hk, r0, n, comp)) return;
     const int linhas = n * Gq, rho0 = tile * RW, i_lo = comp - n + rho0 / Gq, i_hi = comp - n + min(rho0 + RW - 1, linhas - 1) / Gq;
     const Tiles<TK> tl(a, i_lo, i_hi);
     const int rho = rho0 + 16 * w + lr, w_hi = comp - n + min(rho0 + 16 * w + 15, linhas - 1) / Gq;   // w_hi: the wave's last position
@@ -648,59 +717,47 @@ __global__ void __launch_bounds__(64 * NW) k_atc_mf(atc::Args a, int por_seq) {
         for (int z = 0; z < 8; z++) q[k][z] = (__bf16)(e * (float)(int8_t)(x >> (8 * z)));
     }
 
-    const int pag = 1 << a.L.lgpag;
+    // Staging: a thread's chunks of VB bytes, key `chave` and its value. A tile's 16 keys 16 x .. lie in one page (pages hold 16 or
+    // more), so where a wave's keys do too its entry is one scalar read.
+    const int pag = 1 << a.L.lgpag, cc = threadIdx.x % LPK;
     const long long dvm = (long long)a.Hk * pag * HD, dve = (long long)a.Hk * pag * G;        // from a key to its value
-    int pg[IT], de[2][IT], ruim = -1;
+    constexpr bool UMA = 64 / LPK <= 16;
+    int pg[IT], ruim = -1;
+    int8_t de[2][IT];
     int4 dm[2][IT];
-    auto chave = [&](int x) { return (int)(threadIdx.x + 64 * NW * x) / LPK; };
-    // A tile lies in one page where pages hold 64 slots or more: one scalar table read, and a thread's chunk is at a fixed offset
-    // of the tile. Smaller pages are looked up key by key.
-    const bool uma = pag >= TK;
+    bool conta[IT];
+    auto chave = [&](int x) { return min((int)(threadIdx.x + 256 * x) / LPK, TK - 1); };
     auto le_paginas = [&](int t) {
-        if (uma) {
-            const int j0 = tl.j0(t), j = min(max(j0, j0 >= tl.prim * TK ? tl.lo : 0), i_hi);  // a key of the tile that some row sees
-            pg[0] = t < tl.t1 ? __builtin_amdgcn_readfirstlane(a.L.tab[(long long)b * a.L.P + (j >> a.L.lgpag)]) : OCULTA;
-            if (t < tl.t1 && (unsigned)pg[0] >= (unsigned)a.L.npag) { ruim = j; pg[0] = OCULTA; }
-            return;
-        }
-#pragma unroll
-        for (int x = 0; x < IT; x++) pg[x] = (int)threadIdx.x + 64 * NW * x < NT ? pagina(a, tl, b, t, tl.j0(t) + chave(x), i_hi, ruim) : OCULTA;
-    };
-    auto le_dados = [&](int t) {
-        const int j0 = tl.j0(t), cc = threadIdx.x % LPK;
-        const long long base = (long long)hk * pag + (j0 & (pag - 1));
-        const int p0 = __builtin_amdgcn_readfirstlane(pg[0]);
-        const int8_t *m0 = a.cm + p0 * a.pag_m + base * HD, *e0 = a.cE + p0 * a.pag_e + base * G;
 #pragma unroll
         for (int x = 0; x < IT; x++) {
-            dm[0][x] = dm[1][x] = make_int4(0, 0, 0, 0);
-            de[0][x] = de[1][x] = -127;
-            const int key = chave(x), j = j0 + key;
-            if (uma) {
-                if (p0 != OCULTA && (int)threadIdx.x + 64 * NW * x < NT && j <= i_hi && (j >= tl.lo || j < tl.ns)) {
-                    const int8_t *p = m0 + (threadIdx.x + 64 * NW * x) * VB, *e = e0 + key * G + cc * VB / GS;
-                    dm[0][x] = le_vb<VB>(p);
-                    dm[1][x] = le_vb<VB>(p + dvm);
-                    de[0][x] = e[0];
-                    de[1][x] = e[dve];
-                }
-            } else if (pg[x] != OCULTA) {
-                const long long vaga = (long long)hk * pag + (j & (pag - 1));
-                const int8_t *p = a.cm + pg[x] * a.pag_m + vaga * HD + cc * VB, *e = a.cE + pg[x] * a.pag_e + vaga * G + cc * VB / GS;
-                dm[0][x] = le_vb<VB>(p);
-                dm[1][x] = le_vb<VB>(p + dvm);
-                de[0][x] = e[0];
-                de[1][x] = e[dve];
-            }
+            const int j = tl.j0(min(t, tl.t1 - 1)) + chave(x);
+            pg[x] = entrada(a, b, UMA ? __builtin_amdgcn_readfirstlane(j) : j, i_hi);
+        }
+    };
+    auto le_dados = [&](int t) {
+#pragma unroll
+        for (int x = 0; x < IT; x++) {
+            const int j = tl.j0(t) + chave(x);
+            bool ok;
+            const int p = pagina(a, UMA ? __builtin_amdgcn_readfirstlane(pg[x]) : pg[x], ok);
+            const bool vis = visivel(tl, t, j, i_hi);
+            ruim = vis && !ok ? j : ruim;
+            conta[x] = vis && ok;
+            const long long vaga = (long long)hk * pag + (j & (pag - 1));
+            const int8_t *m = a.cm + p * a.pag_m + vaga * HD + cc * VB, *e = a.cE + p * a.pag_e + vaga * G + cc * VB / GS;
+            dm[0][x] = le_vb<VB>(m);
+            dm[1][x] = le_vb<VB>(m + dvm);
+            de[0][x] = e[0];
+            de[1][x] = e[dve];
         }
     };
     auto guarda = [&](int buf) {
 #pragma unroll
         for (int x = 0; x < IT; x++) {
-            if ((int)threadIdx.x + 64 * NW * x >= NT) continue;
-            const int o = chave(x) * VS + threadIdx.x % LPK * VB;
-            valor_lds<VB>(&sk[buf][o], dm[0][x], __builtin_ldexpf(1.f, de[0][x]));
-            valor_lds<VB>(&sv[buf][o], dm[1][x], __builtin_ldexpf(1.f, de[1][x]));
+            if ((int)threadIdx.x + 256 * x >= NT) continue;
+            const int o = chave(x) * VS + cc * VB;
+            valor_lds<VB>(&sk[buf][o], dm[0][x], escala(de[0][x], conta[x]));
+            valor_lds<VB>(&sv[buf][o], dm[1][x], escala(de[1][x], conta[x]));
         }
     };
 
@@ -716,36 +773,35 @@ __global__ void __launch_bounds__(64 * NW) k_atc_mf(atc::Args a, int por_seq) {
         const int buf = (t - tl.t0) & 1, j0 = tl.j0(t);
         if (t + 1 < tl.t1) { le_dados(t + 1); le_paginas(t + 2); }
         if (tem && j0 <= w_hi) {
-            float s[16];
             f4_t x[4];
             const float bias = -incl * (float)(i - j0 - 4 * c);       // the product starts from the bias of each key
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++) {
+            for (int k = 0; k < 16; k++) x[k / 4][k % 4] = __builtin_fmaf(incl, (float)(16 * (k / 4) + k % 4), bias);
 #pragma unroll
-                for (int k = 0; k < 4; k++) x[kt][k] = __builtin_fmaf(incl, (float)(16 * kt + k), bias);
+            for (int kt = 0; kt < 4; kt++)
 #pragma unroll
                 for (int k = 0; k < NM; k++) {
                     b8_t kf = b8_t{};
                     if (HD >= 32 || c < 2) kf = *reinterpret_cast<const b8_t*>(&sk[buf][(16 * kt + lr) * VS + 32 * k + 8 * c]);
                     x[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[k], x[kt], 0, 0, 0);
                 }
-            }
             pronto(x);
+            float s[16];
 #pragma unroll
             for (int k = 0; k < 16; k++) s[k] = x[k / 4][k % 4];
-            // every key of the tile visible to every row of the workgroup: nothing to mask
+            // where every key of the tile is visible to every row of the workgroup there is nothing to mask
             if (j0 + TK - 1 > i_lo || (a.janela > 0 && j0 <= i_hi - a.janela && j0 + TK > a.sumid)) {
                 const int janela = a.janela > 0 ? a.janela : 0x7fffffff;
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
                     const int j = j0 + 4 * c + 16 * (k / 4) + k % 4;
-                    s[k] = j <= i && (i - j < janela || j < a.sumid) ? s[k] : -INFINITY;
+                    s[k] = (j <= i) & ((i - j < janela) | (j < a.sumid)) ? s[k] : -INFINITY;
                 }
             }
             i4_t p[3][2];
             y.pesos(s, p, K);
 #pragma unroll
-            for (int kk = 0; kk < 2; kk++) y.template soma_v<VS>(&sv[buf][32 * kk * VS], p[0][kk], p[1][kk], p[2][kk], lr, c);
+            for (int kk = 0; kk < 2; kk++) soma_v<HD, VS>(y, &sv[buf][32 * kk * VS], p, kk, lr, c);
         }
         if (t + 1 < tl.t1) guarda(buf ^ 1);
         __syncthreads();
@@ -773,49 +829,49 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
     __bf16* sv = reinterpret_cast<__bf16*>(mem + w * (BV + BF));
     float* sf = reinterpret_cast<float*>(mem + w * (BV + BF) + BV);
     int r0, n, comp;
-    if (!linhas_de<HD>(a, blockIdx.x, 0, 1, 16, hk, r0, n, comp)) return;
+    if (!linhas_de<HD>(a, blockIdx.x, true, 0, 1, hk, r0, n, comp)) return;
     const int b = blockIdx.x, linhas = n * Gq, i_lo = comp - n, i_hi = comp - 1, pag = 1 << a.L.lgpag;
     const Tiles<TK> tl(a, i_lo, i_hi);
     const Linha<HD, GS> q(a, r0, n, comp, hk, min(lr, linhas - 1), c);
 
-    // a lane's keys: lr and 16 + lr of the tile for the products; lane / LPK, then 64 / LPK further on, for the values
-    int pk[2], pv[IT], ke[2], ruim = -1;
+    // The tile's first and second 16 keys lie in one page each: two scalar table reads. A lane's keys: lr and 16 + lr for the
+    // products; lane / LPK, then 64 / LPK further on, for the values. Keys are read again once the products have taken them, values
+    // once they are in LDS.
+    constexpr int KV = 64 / LPK;
+    int pg[2], p0[2], ruim = -1;
+    int8_t ke[2], ve[IT];
+    bool ok[2];
     long kf[2][NM];
     int4 dv[IT];
-    int ve[IT];
     auto le_paginas = [&](int t) {
 #pragma unroll
-        for (int k = 0; k < 2; k++) pk[k] = pagina(a, tl, b, t, tl.j0(t) + 16 * k + lr, i_hi, ruim);
-#pragma unroll
-        for (int x = 0; x < IT; x++) {
-            const int key = lane / LPK + 64 / LPK * x;
-            pv[x] = key < TK ? pagina(a, tl, b, t, tl.j0(t) + key, i_hi, ruim) : OCULTA;
-        }
+        for (int k = 0; k < 2; k++) pg[k] = entrada(a, b, __builtin_amdgcn_readfirstlane(tl.j0(min(t, tl.t1 - 1)) + 16 * k), i_hi);
     };
-    auto le_dados = [&](int t) {
+    auto acha_paginas = [&](int t) {
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-#pragma unroll
-            for (int x = 0; x < NM; x++) kf[k][x] = 0;
-            ke[k] = -127;
-            if (pk[k] != OCULTA) {
-                const long long vaga = (long long)hk * pag + ((tl.j0(t) + 16 * k + lr) & (pag - 1));
-                const int8_t* p = a.cm + pk[k] * a.pag_m + vaga * HD;
-#pragma unroll
-                for (int x = 0; x < NM; x++) kf[k][x] = fragmento<HD>(p, x, c);
-                if (c < G) ke[k] = a.cE[pk[k] * a.pag_e + vaga * G + c];
-            }
+            p0[k] = pagina(a, __builtin_amdgcn_readfirstlane(pg[k]), ok[k]);
+            const int j = tl.j0(t) + 16 * k + lr;
+            ruim = !ok[k] && visivel(tl, t, j, i_hi) ? j : ruim;
         }
+    };
+    auto vaga = [&](int t, int key) { return (long long)hk * pag + ((tl.j0(t) + key) & (pag - 1)); };
+    auto le_chaves = [&](int t) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const long long v = vaga(t, 16 * k + lr);
+#pragma unroll
+            for (int x = 0; x < NM; x++) kf[k][x] = fragmento<HD>(a.cm + p0[k] * a.pag_m + v * HD, x, c);
+            ke[k] = a.cE[p0[k] * a.pag_e + v * G + min(c, G - 1)];
+        }
+    };
+    auto le_valores = [&](int t) {
 #pragma unroll
         for (int x = 0; x < IT; x++) {
-            const int key = lane / LPK + 64 / LPK * x, cc = lane % LPK;
-            dv[x] = make_int4(0, 0, 0, 0);
-            ve[x] = -127;
-            if (pv[x] != OCULTA) {
-                const long long vaga = ((long long)a.Hk + hk) * pag + ((tl.j0(t) + key) & (pag - 1));
-                dv[x] = le_vb<VB>(a.cm + pv[x] * a.pag_m + vaga * HD + cc * VB);
-                ve[x] = a.cE[pv[x] * a.pag_e + vaga * G + cc * VB / GS];
-            }
+            const int key = min(lane / LPK + KV * x, TK - 1), cc = lane % LPK, p = KV <= 16 ? p0[KV * x / 16] : key < 16 ? p0[0] : p0[1];
+            const long long v = (long long)a.Hk * pag + vaga(t, key);
+            dv[x] = le_vb<VB>(a.cm + p * a.pag_m + v * HD + cc * VB);
+            ve[x] = a.cE[p * a.pag_e + v * G + cc * VB / GS];
         }
     };
 
@@ -823,40 +879,43 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
     int t = tl.t0 + w;
     if (t < tl.t1) {
         le_paginas(t);
-        le_dados(t);
+        acha_paginas(t);
+        le_chaves(t);
+        le_valores(t);
         le_paginas(t + 4);
     }
     for (; t < tl.t1; t += 4) {
-        const int j0 = tl.j0(t);
-        long k0[2][NM];
+        const int j0 = tl.j0(t), prox = min(t + 4, tl.t1 - 1);
+        const bool cheia = j0 + TK - 1 <= i_hi && (j0 >= tl.lo || j0 + TK <= tl.ns);          // some row sees each of its keys
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            if (c < G) sf[c * TK + 16 * k + lr] = __builtin_ldexpf(1.f, ke[k]);
-#pragma unroll
-            for (int x = 0; x < NM; x++) k0[k][x] = kf[k][x];
-        }
+        for (int k = 0; k < 2; k++)
+            if (c < G) sf[c * TK + 16 * k + lr] = escala(ke[k], ok[k] & (cheia | visivel(tl, t, j0 + 16 * k + lr, i_hi)));
 #pragma unroll
         for (int x = 0; x < IT; x++) {
-            const int key = lane / LPK + 64 / LPK * x;
-            if (key < TK) valor_lds<VB>(sv + key * VS + lane % LPK * VB, dv[x], __builtin_ldexpf(1.f, ve[x]));
+            const int key = lane / LPK + KV * x;
+            const bool bom = KV <= 16 ? ok[KV * x / 16 % 2] : key < 16 ? ok[0] : ok[1];
+            if (key < TK) valor_lds<VB>(sv + key * VS + lane % LPK * VB, dv[x], escala(ve[x], bom & (cheia | visivel(tl, t, j0 + key, i_hi))));
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (t + 4 < tl.t1) { le_dados(t + 4); le_paginas(t + 8); }
+        acha_paginas(prox);
+        le_valores(prox);
         float s[8];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             float4 f[G];
 #pragma unroll
             for (int g = 0; g < G; g++) f[g] = *reinterpret_cast<const float4*>(sf + g * TK + 16 * k + 4 * c);
-            q.notas(k0[k], f, j0 + 16 * k + 4 * c, s + 4 * k);
+            q.notas(kf[k], f, j0 + 16 * k + 4 * c, s + 4 * k);
         }
+        le_chaves(prox);
+        le_paginas(t + 8);
         if (j0 + TK - 1 > i_lo || (a.janela > 0 && j0 <= i_hi - a.janela && j0 + TK > a.sumid)) {
 #pragma unroll
             for (int k = 0; k < 8; k++) s[k] = q.ve(a, j0 + 16 * (k / 4) + 4 * c + k % 4) ? s[k] : -INFINITY;
         }
         i4_t p[3][1];
         y.pesos(s, p);
-        y.template soma_v<VS>(sv, p[0][0], p[1][0], p[2][0], lr, c);
+        soma_v<HD, VS>(y, sv, p, 0, lr, c);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     relata_pagina(a, b, ruim);
