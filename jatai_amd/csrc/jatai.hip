@@ -1045,46 +1045,34 @@ int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, in
     return 0;
 }
 
-// How a call runs, by the rows that share a kv head's keys at most: one (k_atc_um, a row per workgroup), up to 16 (k_atc_gr) or
-// more (k_atc_mf, 64 rows a workgroup). S splits of the visible tokens, `fatia` tokens (um) or
-// tiles of 32 (gr) or 64 (mf) tokens each: as many as fill the chip, each with at least one step of a workgroup's loop (um), two
-// tiles a wave (gr) or four tiles (mf). direto: one split, and every block of the output lies in a head, so the kernel
-// writes it and there is no join.
+// How a call runs, by the rows that share a kv head's keys at most: one (k_atc_um, a row per workgroup; 64-wide heads, 4 sequences
+// of 90,001 to 131,071 tokens: 94 us, 112 in k_atc_gr; 16 sequences of up to 2050 tokens, 64 heads of 4: 14 and 33), up to 16
+// (k_atc_gr; 32 query heads on 8 of 128, 64 sequences of up to 4096 tokens: 88 us, 210 in k_atc_mf, 184 row by row) or more
+// (k_atc_mf, 64 rows a workgroup). S splits of the visible tokens, `fatia` tiles each. One token at a time the workgroups should
+// number two per CU, with at least one tile a wave (um) or two (gr): a row's work is all reading, and every workgroup more costs
+// its start, its end and its part of the join (long contexts above at 512, 1024, 2048 workgroups 94, 101, 99 us; 64 sequences in a
+// window of 1024 19, 25, 27). Rows of prompts, 1024 workgroups, at least four tiles each and at most 24, so that the longest row
+// does not outlast the others (8 prompts of up to 4000 tokens at 12, 24, 40 tiles and undivided: 208, 190, 200 and 239 us).
+// direto: one split, and every block of the output lies in a head, so the kernel writes it and there is no join.
 enum { ATC_UM, ATC_GR, ATC_MF };
-#ifndef ATC_UMAX
-#define ATC_UMAX 1
-#endif
-#ifndef ATC_ALVO
-#define ATC_ALVO 2048
-#endif
-#ifndef ATC_FATIA
-#define ATC_FATIA 24
-#endif
 struct PlanoAtc { int tipo; bool direto; unsigned tiles; int S, fatia; };
 static PlanoAtc atc_plano(long long M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo) {
     PlanoAtc p;
-    const long long linhas = (long long)novos * (H / Hk);
-        p.tipo = linhas > 16 ? ATC_MF : linhas > ATC_UMAX ? ATC_GR : ATC_UM;
+    const long long linhas = (long long)novos * (H / Hk), por_wg = 64;
+    p.tipo = linhas > 16 ? ATC_MF : linhas > 1 ? ATC_GR : ATC_UM;
     const bool mf = p.tipo == ATC_MF;
-    const long long por_wg = 64;
-    // every sequence's tiles (its last one may be cut short), and one workgroup at least for the rows of no sequence
+    // every sequence's tiles of rows (its last one may be cut short), and one workgroup at least for the rows of no sequence
     p.tiles = (unsigned)std::min((M * (H / Hk) + por_wg - 1) / por_wg + B + 1, 0x7fffffffLL);
-    long long nv = std::max(1LL, janela > 0 ? std::min((long long)teto, (long long)janela + sumid) : (long long)teto), passo, wgs, alvo = ATC_ALVO;
-    if (p.tipo == ATC_UM) {
-        passo = hd <= 16 ? 1024 : 16384 / hd;
-        wgs = M * H;
-    } else {                                                         // in tiles: a window's may begin and end inside one, the first tokens' too
-        const long long tk = mf ? 64 : 32, nt = (teto + tk - 1) / tk;
-        nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, por_wg) + tk - 2) / tk + 1 + (sumid + tk - 1) / tk) : nt);
-        passo = mf ? 4 : 8;
-        if (mf) alvo = 1024;
-        wgs = (mf ? (M * (H / Hk) + por_wg - 1) / por_wg : (long long)B) * Hk;
-    }
+    // tokens of a tile: a wave's four loads (um), 32 (gr), 64 (mf); a window's tokens may begin and end inside one, the first tokens too
+    const long long tk = mf ? 64 : p.tipo == ATC_GR ? 32 : hd <= 16 ? 256 : 4096 / hd, nt = (teto + tk - 1) / tk;
+    const long long nv = std::max(1LL, janela > 0 ? std::min(nt, (janela + std::min((long long)novos, por_wg) + tk - 2) / tk + 1 + (sumid + tk - 1) / tk) : nt);
+    const long long passo = p.tipo == ATC_GR ? 8 : 4, alvo = mf ? 1024 : 512;
+    const long long wgs = mf ? (M * (H / Hk) + por_wg - 1) / por_wg * Hk : p.tipo == ATC_GR ? (long long)B * Hk : M * H;
     long long s = std::min(std::max(alvo / std::max(wgs, 1LL), 1LL), (nv + passo - 1) / passo);
-    if (mf) s = std::max(s, (nv + ATC_FATIA - 1) / ATC_FATIA);
+    if (mf) s = std::max(s, (nv + 23) / 24);
     p.fatia = (int)(((nv + s - 1) / s + passo - 1) / passo * passo);
     p.S = (int)((nv + p.fatia - 1) / p.fatia);
-    p.direto = p.tipo != ATC_UM && p.S == 1 && (tipo != 0 || hd >= g_blk);
+    p.direto = p.S == 1 && (tipo != 0 || hd >= g_blk);
     return p;
 }
 long long jt_atencao_cache_ws_bytes(int M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo) {
@@ -1116,8 +1104,8 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
     int rc = fim();
     if (rc || p.direto) return rc;
     const int C = H * hd;
-    const dim3 grade(M, (C + 127) / 128);
-#define J(BL, T) (p.S <= 8 ? k_atc_junta<BL, T, 2><<<grade, 64, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)       \
+    const dim3 grade(M, p.S <= 8 ? (C + 511) / 512 : (C + 127) / 128);
+#define J(BL, T) (p.S <= 8 ? k_atc_junta<BL, T, 2><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)       \
                   : p.S <= 32 ? k_atc_junta<BL, T, 8><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)   \
                               : k_atc_junta<BL, T, 32><<<grade, 1024, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid))
     if (tipo == 1) J(32, 1);
@@ -1166,14 +1154,14 @@ int jt_gemv4(const void* x, const void* xE, const void* w4, const void* esc, con
     if (M < 0 || N <= 0 || K <= 0 || K % g_blk || K > 256 * g_blk || modo < 0 || modo > 3 || (modo != 1 && N % g_blk)) return (int)hipErrorInvalidValue;
     if (M == 0) return 0;
     if (!x || !xE || !w4 || !esc || !R || !y || !yE || !alinhados(x, w4, esc, R, y, yE) || (modo == 2 && (!res || !resE || !alinhado(res)))) return (int)hipErrorInvalidValue;
-    const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4, Kt = (K + 127) / 128, cg = modo == 1 ? 1 : g_blk / COLS, ks = std::min(Kt, (mt == 4 ? 8 : 16) / cg);
+    const int mt = M <= 16 ? 1 : 2, Kt = (K + 127) / 128, cg = modo == 1 ? 1 : g_blk / COLS, ks = std::min(Kt, (mt > 1 ? 8 : 16) / cg);
     const Args a{(const int8_t*)x, (const int8_t*)xE, (const int4*)w4, (const uint16_t*)esc, (const int16_t*)R, (const int8_t*)res, (const int8_t*)resE,
                  y, yE, M, N, K, modo, ks, cg, kid};
     const dim3 grade((N + COLS * cg - 1) / (COLS * cg), (M + 16 * mt - 1) / (16 * mt));
     if (grade.y > 65535) return (int)hipErrorInvalidValue;
-    const size_t lds = 4 * ((size_t)K / g_blk * 16 * mt + 16 * mt + (size_t)16 * mt * COLS * cg);
+    const size_t lds = 4 * ((size_t)K / g_blk * 16 * mt + 16 * mt + (size_t)16 * mt * COLS * cg) + (size_t)ks * cg * 16 * mt * 144;
 #define L(BL, NR, MT) (lds_max(k_gemv4<BL, NR, MT>, lds), k_gemv4<BL, NR, MT><<<grade, 64 * ks * cg, lds, g_stream>>>(a))
-#define LM(BL) (M <= 4 ? L(BL, 1, 1) : M <= 8 ? L(BL, 2, 1) : M <= 16 ? L(BL, 4, 1) : M <= 32 ? L(BL, 4, 2) : L(BL, 4, 4))
+#define LM(BL) (M <= 4 ? L(BL, 1, 1) : M <= 8 ? L(BL, 2, 1) : M <= 16 ? L(BL, 4, 1) : L(BL, 4, 2))
     if (g_blk == 32) LM(32);
     else LM(128);
 #undef LM

@@ -42,11 +42,31 @@ __device__ __forceinline__ int sequencia_de(const Lote& L, int r) {
     return n - 1 >= 0 && r < L.ini[n] ? n - 1 : -1;
 }
 
+// the same with the sequence's own numbers, which the lanes load beside the starts: still one round trip
 __device__ __forceinline__ Seq acha(const Lote& L, int r, int kid, bool relata) {
-    Seq s{sequencia_de(L, r), 0, 0};
+    Seq s{-1, 0, 0};
+    int r0 = r, fim = r + 1, comp = 0;
+    if (L.ini) {
+        for (int k = 0; k < L.B; k += 64) {
+            const int x = k + (int)(threadIdx.x & 63), a = L.ini[min(x, L.B)], b = L.ini[min(x + 1, L.B)], c = L.comp[min(x, L.B - 1)];
+            const int n = __popcll(__ballot(x < L.B && a <= r));
+            if (n == 0) break;
+            s.b = k + n - 1;
+            r0 = __shfl(a, n - 1);
+            fim = __shfl(b, n - 1);
+            comp = __shfl(c, n - 1);
+            if (n < 64) break;
+        }
+        if (r >= fim) s.b = -1;
+    } else if (r < L.B) {
+        s.b = r;
+        comp = L.comp[r];
+        fim = r + min(comp, 1);                                       // an empty sequence has no row
+    }
     if (s.b < 0) return s;
-    int r0, n, comp;
-    s.ok = sequencia(L, s.b, r0, n, comp, kid, relata);
+    const int n = fim - r0;
+    s.ok = r0 >= 0 && n >= 0 && r0 <= L.M - n && n <= L.novos && comp >= n && comp <= L.teto;
+    if (!s.ok && relata) reporta(E_ARG, kid, r0, comp, s.b);
     s.ok = s.ok && r - r0 < n;
     s.i = comp - n + (r - r0);
     return s;
@@ -116,7 +136,7 @@ struct Args {
     long long pag_m, pag_e;
     Lote L;
     bool inteira;                                // the blocks of a block output lie in one head each
-    int H, Hk, lgblk, janela, sumid, S, fatia, tipo, kid;   // S splits of `fatia` visible tokens (k_atc_gr, k_atc_mf: tiles) each
+    int H, Hk, lgblk, janela, sumid, S, fatia, tipo, kid;   // S splits of `fatia` tiles of visible tokens each
 };
 
 // a page outside the cache that the token at position `ruim` (-1: none) of sequence b needed
@@ -152,138 +172,6 @@ __device__ __forceinline__ float soma_grupo(float v) {               // over LPK
 }
 }  // namespace atc
 
-// One row (token, query head) and one split of its visible tokens per workgroup. Softmax in one pass: every group of LPK
-// lanes (a key's head row, 16 bytes a lane) keeps the running maximum m, sum l and output o of the keys it has seen,
-//   u = 2^(Eq + Ek) (mq . mk) / sqrt(hd) - incl (i - j);  p = exp(u - m);  o += p 2^Ev mv,
-// and they are joined at the end (lanes, waves, then the splits by k_atc_junta). Products of mantissas are exact in int32
-// (v_dot4), statistics and outputs fp32. The visible tokens are numbered x = 0 .. nvis - 1 without gaps, the first tokens
-// then the window, so no masked key is read.
-template <int HD, int GS>
-__global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
-    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, KPW = 64 / LPK, U = 4, NW = 4, G = HD / GS;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane % LPK;
-    const int r = blockIdx.x, h = blockIdx.y, s = blockIdx.z, hk = h / (a.H / a.Hk), g = c * VB / GS;
-    const atc::Seq q = atc::acha(a.L, r, a.kid, threadIdx.x == 0 && h == 0 && s == 0);
-    int nvis = 0, ns = 0, lo = 0;
-    if (q.ok) {
-        lo = a.janela > 0 ? max(0, q.i + 1 - a.janela) : 0;
-        ns = min(a.sumid, lo);
-        nvis = ns + q.i + 1 - lo;
-    }
-    const int x0 = min((long long)s * a.fatia, (long long)nvis), x1 = min(x0 + a.fatia, nvis), pag = 1 << a.L.lgpag;
-
-    int qv[VB / 4];
-    const int ld = (a.H + 2 * a.Hk) * HD, col = h * HD + c * VB;
-#pragma unroll
-    for (int k = 0; k < VB / 4; k++) qv[k] = reinterpret_cast<const int*>(a.qm + (long long)r * ld + col)[k];
-    const int eq = a.qE[(long long)r * (ld >> a.lgblk) + (col >> a.lgblk)];
-    const float esc = 1.f / __builtin_sqrtf((float)HD), incl = a.incl ? a.incl[h] : 0.f;
-
-    float m = -INFINITY, l = 0.f, o[VB];
-#pragma unroll
-    for (int d = 0; d < VB; d++) o[d] = 0.f;
-    const long long dv = (long long)a.Hk * pag;                        // slots between a token's key and its value
-    int ruim = -1;
-    for (int base = x0 + w * KPW * U; base < x1; base += NW * KPW * U) {
-        int j[U], p[U];
-        bool vis[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int x = base + u * KPW + lane / LPK, xx = min(x, x1 - 1);
-            vis[u] = x < x1;
-            j[u] = xx < ns ? xx : xx - ns + lo;
-            p[u] = a.L.tab[(long long)q.b * a.L.P + (j[u] >> a.L.lgpag)];
-        }
-        int kv[U][VB / 4], vv[U][VB / 4], ek[U], ev[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const bool fora = (unsigned)p[u] >= (unsigned)a.L.npag;
-            ruim = vis[u] && fora ? j[u] : ruim;
-            vis[u] = vis[u] && !fora;
-            p[u] = fora ? 0 : p[u];
-            const long long vaga = (long long)hk * pag + (j[u] & (pag - 1));
-            const int8_t *km = a.cm + p[u] * a.pag_m + vaga * HD + c * VB, *ke = a.cE + p[u] * a.pag_e + vaga * G + g;
-#pragma unroll
-            for (int k = 0; k < VB / 4; k++) {
-                kv[u][k] = reinterpret_cast<const int*>(km)[k];
-                vv[u][k] = reinterpret_cast<const int*>(km + dv * HD)[k];
-            }
-            ek[u] = ke[0];
-            ev[u] = ke[dv * G];
-        }
-        float t[U], mn = m;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            int d = 0;
-#pragma unroll
-            for (int k = 0; k < VB / 4; k++) d = __builtin_amdgcn_sdot4(qv[k], kv[u][k], d, false);
-            t[u] = atc::soma_grupo<LPK>(__builtin_ldexpf((float)d, eq + ek[u])) * esc - incl * (float)(q.i - j[u]);
-            t[u] = vis[u] ? t[u] : -INFINITY;
-            mn = fmaxf(mn, t[u]);
-        }
-        const float mL = mn == -INFINITY ? 0.f : atc::vezes(mn, atc::LOG2E), al = atc::fator(m, mn);
-        m = mn;
-        l *= al;
-#pragma unroll
-        for (int d = 0; d < VB; d++) o[d] *= al;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const float e = atc::peso(t[u], mL);
-            l += e;
-            const float pv = vis[u] ? __builtin_ldexpf(e, ev[u]) : 0.f;
-#pragma unroll
-            for (int d = 0; d < VB; d++) o[d] += pv * (float)(int8_t)(vv[u][d / 4] >> (8 * (d % 4)));
-        }
-    }
-
-    atc::relata_pagina(a, q.b, ruim);
-
-    // the wave's groups: a common maximum, then sums in which every step halves the values a lane still holds
-    float M = m;
-#pragma unroll
-    for (int x = LPK; x < 64; x *= 2) M = fmaxf(M, __shfl_xor(M, x));
-    const float es = atc::fator(m, M);
-    l *= es;
-#pragma unroll
-    for (int x = LPK; x < 64; x *= 2) l += __shfl_xor(l, x);
-#pragma unroll
-    for (int d = 0; d < VB; d++) o[d] *= es;
-    int d0 = 0;
-#pragma unroll
-    for (int x = LPK, n = VB; x < 64; x *= 2) {
-        if (n > 1) {
-            n /= 2;
-            const bool alto = lane & x;
-#pragma unroll
-            for (int d = 0; d < VB / 2; d++)
-                if (d < n) {
-                    const float fica = alto ? o[d + n] : o[d], vai = alto ? o[d] : o[d + n];
-                    o[d] = fica + __shfl_xor(vai, x);
-                }
-            d0 += alto ? n : 0;
-        } else o[0] += __shfl_xor(o[0], x);
-    }
-    constexpr int RESTO = VB / KPW > 1 ? VB / KPW : 1;                 // values a lane is left with
-    __shared__ float so[NW][HD], sm[NW], sl[NW];
-#pragma unroll
-    for (int d = 0; d < RESTO; d++) so[w][c * VB + d0 + d] = o[d];     // lanes with the same values write the same
-    if (lane == 0) { sm[w] = M; sl[w] = l; }
-    __syncthreads();
-    if (threadIdx.x >= HD) return;
-    float MM = sm[0], LL = 0.f, oo = 0.f;
-#pragma unroll
-    for (int k = 1; k < NW; k++) MM = fmaxf(MM, sm[k]);
-#pragma unroll
-    for (int k = 0; k < NW; k++) {
-        const float f = atc::fator(sm[k], MM);
-        LL += sl[k] * f;
-        oo += so[k][threadIdx.x] * f;
-    }
-    const long long part = ((long long)r * a.H + h) * a.S + s;
-    a.o[part * HD + threadIdx.x] = oo;
-    if (threadIdx.x == 0) { a.ml[2 * part] = MM; a.ml[2 * part + 1] = LL; }
-}
-
 // Exponent of a block of fp32 values in the int8 format, from the bits of the largest |v|, and the scale 2^-E: E = binary
 // exponent - 7, one up where the largest mantissa rounds past 127 (half to even; products by 2^-E are exact). A block below
 // 2^-126 is zero; one that holds an infinity or a NaN raises E_EXP and is zero.
@@ -307,17 +195,36 @@ __device__ __forceinline__ int quant_f32(const float (&v)[NV], int8_t (&q)[NV], 
     return E;
 }
 
+// 4 values of a row from position x on, as a block tensor (blocks of BLK values, whose lanes write together), bfloat16 or fp32
+template <int BLK>
+__device__ __forceinline__ void grava_4(void* out, int8_t* outE, int tipo, long long x, const float (&v)[4], int kid) {
+    if (tipo == 0) {
+        if constexpr (BLK >= 32) {
+            int8_t q[4];
+            const int E = quant_f32<4, BLK / 4>(v, q, kid, x);
+            grava_i8<4, false>((int8_t*)out + x, q);
+            if (x % BLK == 0) outE[x / BLK] = (int8_t)E;
+        }
+    } else if (tipo == 1) {
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<b4*>((__bf16*)out + x) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    } else {
+        *reinterpret_cast<float4*>((float*)out + x) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+
 // Joins the splits of a row and head, o = sum exp(m_s - m) o_s / sum exp(m_s - m) l_s (zeros for a row without visible
-// tokens), and writes the row as a block tensor (TIPO 0), bfloat16 (1) or fp32 (2). A workgroup takes 128 columns of a row, 4 a
-// thread, and shares the splits out among its NG groups of 32 threads, four of them in flight at a time: one
-// thread walking 64 splits one by one waited for each (30 us of a call of 131).
+// tokens), and writes the row as a block tensor (TIPO 0), bfloat16 (1) or fp32 (2). NG groups of 32 threads share out the splits
+// of 128 columns of a row, 4 columns a thread, four splits in flight at a time: one thread walking 64 splits one by one
+// waited for each (30 us of a call of 131). With NG = 2 the groups are one wave, and a workgroup takes 512 columns in four of them.
 template <int BLK, int TIPO, int NG>
-__global__ void __launch_bounds__(32 * NG) k_atc_junta(const float* __restrict__ ml, const float* __restrict__ po, void* __restrict__ out,
-                                                    int8_t* __restrict__ oE, int C, int hd, int S, int kid) {
-    const int r = blockIdx.x, ct = threadIdx.x & 31, g = threadIdx.x >> 5, col = blockIdx.y * 128 + 4 * ct, cc = min(col, C - 4);
+__global__ void __launch_bounds__(NG == 2 ? 256 : 32 * NG) k_atc_junta(const float* __restrict__ ml, const float* __restrict__ po, void* __restrict__ out,
+                                                                       int8_t* __restrict__ oE, int C, int hd, int S, int kid) {
+    const int r = blockIdx.x, ct = threadIdx.x & 31, g = (threadIdx.x >> 5) % NG, faixa = NG == 2 ? blockIdx.y * 4 + (threadIdx.x >> 6) : blockIdx.y;
+    const int col = faixa * 128 + 4 * ct, cc = min(col, C - 4);
     const long long part = ((long long)r * (C / hd) + cc / hd) * S;
     const bool escrita = ml[2 * part] == INFINITY || col >= C;        // by its one split
-    if (__all(escrita)) return;                                       // every wave has the same columns
+    if (__all(escrita)) return;                                       // the waves that share splits have the same columns
     float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = g; s0 < S; s0 += 4 * NG) {
         float2 x[4];
@@ -345,37 +252,34 @@ __global__ void __launch_bounds__(32 * NG) k_atc_junta(const float* __restrict__
             v[2] += tem ? f * y[k].z : 0.f; v[3] += tem ? f * y[k].w : 0.f;
         }
     }
-    __shared__ float sm[NG][32], sl[NG][32];
-    __shared__ float4 sv[NG][32];
-    sm[g][ct] = M;
-    sl[g][ct] = L;
-    sv[g][ct] = make_float4(v[0], v[1], v[2], v[3]);
-    __syncthreads();
-    if (g > 0 || escrita) return;
-    float MM = M;
-    for (int k = 1; k < NG; k++) MM = fmaxf(MM, sm[k][ct]);
-    L = v[0] = v[1] = v[2] = v[3] = 0.f;
-    for (int k = 0; k < NG; k++) {
-        const float f = atc::fator(sm[k][ct], MM);
-        const float4 x = sv[k][ct];
-        L += f * sl[k][ct];
-        v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+    if constexpr (NG == 2) {
+        const float MM = fmaxf(M, __shfl_xor(M, 32)), f = atc::fator(M, MM);
+        L = L * f + __shfl_xor(L * f, 32);
+#pragma unroll
+        for (int d = 0; d < 4; d++) v[d] = v[d] * f + __shfl_xor(v[d] * f, 32);
+        if (g > 0 || escrita) return;
+    } else {
+        __shared__ float sm[NG][32], sl[NG][32];
+        __shared__ float4 sv[NG][32];
+        sm[g][ct] = M;
+        sl[g][ct] = L;
+        sv[g][ct] = make_float4(v[0], v[1], v[2], v[3]);
+        __syncthreads();
+        if (g > 0 || escrita) return;
+        float MM = M;
+        for (int k = 1; k < NG; k++) MM = fmaxf(MM, sm[k][ct]);
+        L = v[0] = v[1] = v[2] = v[3] = 0.f;
+        for (int k = 0; k < NG; k++) {
+            const float f = atc::fator(sm[k][ct], MM);
+            const float4 x = sv[k][ct];
+            L += f * sl[k][ct];
+            v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+        }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int k = 0; k < 4; k++) v[k] *= inv;
-    const long long x = (long long)r * C + col;
-    if constexpr (TIPO == 0) {
-        int8_t q[4];
-        const int E = quant_f32<4, BLK / 4>(v, q, kid, x);
-        grava_i8<4, false>((int8_t*)out + x, q);
-        if (col % BLK == 0) oE[x / BLK] = (int8_t)E;
-    } else if constexpr (TIPO == 1) {
-        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<b4*>((__bf16*)out + x) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-    } else {
-        *reinterpret_cast<float4*>((float*)out + x) = make_float4(v[0], v[1], v[2], v[3]);
-    }
+    grava_4<BLK>(out, oE, TIPO, (long long)r * C + col, v, kid);
 }
 
 namespace atc {
@@ -674,6 +578,174 @@ __device__ __forceinline__ int4 le_vb(const int8_t* p) {
     else return make_int4(*reinterpret_cast<const int*>(p), 0, 0, 0);
 }
 }  // namespace atc
+
+// One row (token, query head) and one split of its visible tokens per workgroup, the four waves a tile of 4 wave loads each in
+// turn. Softmax in one pass: every group of LPK lanes (a key's head row, 16 bytes a lane) keeps the running maximum m, sum l and
+// output o of the keys it has seen,
+//   u = 2^(Eq + Ek) (mq . mk) / sqrt(hd) - incl (i - j);  p = exp(u - m);  o += p 2^Ev mv,
+// and they are joined at the end (lanes, waves, then the splits by k_atc_junta). Products of mantissas are exact in int32
+// (v_dot4), statistics and outputs fp32. Only the page table is read a tile ahead: holding the next tile's bytes too costs a fifth
+// of the waves and is slower (104 us against 92 below).
+// Reading the keys and values bounds it: 4 sequences of 90,001 to 131,071 tokens, 8 heads of 64.
+template <int HD, int GS>
+__global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
+    using namespace atc;
+    constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, KPW = 64 / LPK, U = 4, NW = 4, G = HD / GS, TK = U * KPW;
+    constexpr bool UMA = KPW <= 16;                                   // a wave load's keys lie in one page
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane % LPK;
+    const int r = blockIdx.x, h = blockIdx.y, hk = h / (a.H / a.Hk), g = c * VB / GS, pag = 1 << a.L.lgpag;
+    const Seq q = acha(a.L, r, a.kid, threadIdx.x == 0 && h == 0 && blockIdx.z == 0);
+    Tiles<TK> tl(a, max(q.i, 0), max(q.i, 0));
+    if (!q.ok) { tl.t0 = tl.t1 = 0; tl.uma = true; }
+
+    int qv[VB / 4];
+    const int ld = (a.H + 2 * a.Hk) * HD, col = h * HD + c * VB;
+#pragma unroll
+    for (int k = 0; k < VB / 4; k++) qv[k] = reinterpret_cast<const int*>(a.qm + (long long)r * ld + col)[k];
+    const int eq = a.qE[(long long)r * (ld >> a.lgblk) + (col >> a.lgblk)];
+    const float esc = 1.f / __builtin_sqrtf((float)HD), incl = a.incl ? a.incl[h] : 0.f;
+
+    const long long dv = (long long)a.Hk * pag;                       // slots between a token's key and its value
+    int pg[U], p0[U], kv[U][VB / 4], vv[U][VB / 4], ruim = -1;
+    int8_t ek[U], ev[U];
+    bool ok[U];
+    auto chave = [&](int t, int u) { return tl.j0(t) + u * KPW + lane / LPK; };
+    auto le_paginas = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = chave(min(t, tl.t1 - 1), u);
+            pg[u] = entrada(a, q.b, UMA ? __builtin_amdgcn_readfirstlane(j) : j, q.i);
+        }
+    };
+    auto acha_paginas = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            p0[u] = pagina(a, UMA ? __builtin_amdgcn_readfirstlane(pg[u]) : pg[u], ok[u]);
+            const int j = chave(t, u);
+            ruim = !ok[u] && visivel(tl, t, j, q.i) ? j : ruim;
+        }
+    };
+    auto vaga = [&](int t, int u) { return (long long)hk * pag + (chave(t, u) & (pag - 1)); };
+    auto le_chaves = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int8_t* m = a.cm + p0[u] * a.pag_m + vaga(t, u) * HD + c * VB;
+#pragma unroll
+            for (int k = 0; k < VB / 4; k++) kv[u][k] = reinterpret_cast<const int*>(m)[k];
+            ek[u] = a.cE[p0[u] * a.pag_e + vaga(t, u) * G + g];
+        }
+    };
+    auto le_valores = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int8_t* m = a.cm + p0[u] * a.pag_m + (dv + vaga(t, u)) * HD + c * VB;
+#pragma unroll
+            for (int k = 0; k < VB / 4; k++) vv[u][k] = reinterpret_cast<const int*>(m)[k];
+            ev[u] = a.cE[p0[u] * a.pag_e + (dv + vaga(t, u)) * G + g];
+        }
+    };
+
+    float m = -INFINITY, l = 0.f, o[VB];
+#pragma unroll
+    for (int d = 0; d < VB; d++) o[d] = 0.f;
+    int t = tl.t0 + w;
+    if (t < tl.t1) le_paginas(t);
+    for (; t < tl.t1; t += NW) {
+        const int j0 = tl.j0(t);
+        acha_paginas(t);
+        le_chaves(t);
+        le_valores(t);
+        le_paginas(t + NW);
+        const bool cheia = (j0 + TK - 1 <= q.i) & ((j0 >= tl.lo) | (j0 + TK <= tl.ns));
+        float s[U], mn = m;
+        bool vis[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = chave(t, u);
+            vis[u] = ok[u] & (cheia | visivel(tl, t, j, q.i));
+            int d = 0;
+#pragma unroll
+            for (int k = 0; k < VB / 4; k++) d = __builtin_amdgcn_sdot4(qv[k], kv[u][k], d, false);
+            s[u] = soma_grupo<LPK>(__builtin_ldexpf((float)d, eq + ek[u])) * esc - incl * (float)(q.i - j);
+            s[u] = vis[u] ? s[u] : -INFINITY;
+            mn = fmaxf(mn, s[u]);
+        }
+        if (__any(mn > m)) {
+            const float al = fator(m, mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < VB; d++) o[d] *= al;
+        }
+        const float mL = m == -INFINITY ? 0.f : vezes(m, LOG2E);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float e = peso(s[u], mL), pv = vis[u] ? __builtin_ldexpf(e, ev[u]) : 0.f;
+            l += e;
+#pragma unroll
+            for (int d = 0; d < VB; d++) o[d] += pv * (float)(int8_t)(vv[u][d / 4] >> (8 * (d % 4)));
+        }
+    }
+    relata_pagina(a, q.b, ruim);
+
+    // the wave's groups: a common maximum, then sums in which every step halves the values a lane still holds
+    float M = m;
+#pragma unroll
+    for (int x = LPK; x < 64; x *= 2) M = fmaxf(M, __shfl_xor(M, x));
+    const float es = fator(m, M);
+    l *= es;
+#pragma unroll
+    for (int x = LPK; x < 64; x *= 2) l += __shfl_xor(l, x);
+#pragma unroll
+    for (int d = 0; d < VB; d++) o[d] *= es;
+    int d0 = 0;
+#pragma unroll
+    for (int x = LPK, n = VB; x < 64; x *= 2) {
+        if (n > 1) {
+            n /= 2;
+            const bool alto = lane & x;
+#pragma unroll
+            for (int d = 0; d < VB / 2; d++)
+                if (d < n) {
+                    const float fica = alto ? o[d + n] : o[d], vai = alto ? o[d] : o[d + n];
+                    o[d] = fica + __shfl_xor(vai, x);
+                }
+            d0 += alto ? n : 0;
+        } else o[0] += __shfl_xor(o[0], x);
+    }
+    constexpr int RESTO = VB / KPW > 1 ? VB / KPW : 1;                // values a lane is left with
+    __shared__ __align__(16) float so[NW][HD];
+    __shared__ float sm[NW], sl[NW];
+#pragma unroll
+    for (int d = 0; d < RESTO; d++) so[w][c * VB + d0 + d] = o[d];    // lanes with the same values write the same
+    if (lane == 0) { sm[w] = M; sl[w] = l; }
+    __syncthreads();
+    if (threadIdx.x >= HD / 4) return;
+    float MM = sm[0], LL = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 1; k < NW; k++) MM = fmaxf(MM, sm[k]);
+#pragma unroll
+    for (int k = 0; k < NW; k++) {
+        const float f = fator(sm[k], MM);
+        const float4 x = *reinterpret_cast<const float4*>(&so[k][4 * threadIdx.x]);
+        LL += sl[k] * f;
+        v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+    }
+    const long long part = ((long long)r * a.H + h) * a.S + blockIdx.z;
+    if (a.ml && !(tl.uma && a.inteira)) {
+        *reinterpret_cast<float4*>(a.o + part * HD + 4 * threadIdx.x) = make_float4(v[0], v[1], v[2], v[3]);
+        if (threadIdx.x == 0) { a.ml[2 * part] = MM; a.ml[2 * part + 1] = LL; }
+        return;
+    }
+    if (a.ml) {                                                       // the row's one split: written here
+        if (blockIdx.z > 0) return;
+        if (threadIdx.x == 0) a.ml[2 * part] = INFINITY;
+    }
+    const float inv = LL == 0.f ? 0.f : 1.f / LL;
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] *= inv;
+    grava_4<GS>(a.out, a.outE, a.tipo, (long long)r * a.H * HD + h * HD + 4 * threadIdx.x, v, a.kid);
+}
 
 // Many rows that share keys and values (new tokens of a sequence, query heads of a group): 16 a wave, 64 per workgroup, on
 // matrix cores; the workgroup walks its keys in tiles of 64. Row rho of a (sequence, kv head) is token rho / Gq,

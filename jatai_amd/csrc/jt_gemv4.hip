@@ -14,6 +14,7 @@
 
 namespace gv4 {
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 constexpr int CT = 2, COLS = 16 * CT;            // column tiles of a wave, and their columns
 
 struct Args {
@@ -34,9 +35,13 @@ constexpr int MAGICO = 0x4B400000;               // bits of 1.5 * 2^23: a float 
 // go to the MFMA as 16 q: the high ones by a mask, the low ones by a shift and a mask. Per result and block: the product as
 // a float (exact), one multiplication for the scale (exact), one FMA onto 1.5 * 2^23 whose single rounding is the block's,
 // and an integer add of its bits. The KS waves add their sums in LDS.
-// 64 rows (MT = 4) hold more than the 128 registers of a 16-wave workgroup: 8 waves there.
+//   What bounds it: the weights' bytes, the rounding close behind (3.3 VALU operations per result and block; 7 us of VALU at
+// 16 rows), and the launch. Every workgroup reads all of X from the L2: as whole lines, 16 bytes a lane, through the wave's own
+// LDS. Read in the MFMA's layout (8 bytes of 16 rows a load, a quarter of each line) X was what bounded it: 16 x 8192 x 8192
+// 16.3 us, 11.2 this way (3.4 TB/s of weights; 9.9 at 4 rows). 16 waves a workgroup, two steps of weights in flight; four, or 8 waves: the same.
+// More than 16 rows hold more registers: two tiles of 16 and 8 waves there (64 rows of 8192 x 8192: 33 us).
 template <int BLK, int NR, int MT>
-__global__ void __launch_bounds__(MT == 4 ? 512 : 1024) k_gemv4(gv4::Args a) {
+__global__ void __launch_bounds__(MT > 1 ? 512 : 1024) k_gemv4(gv4::Args a) {
     using namespace gv4;
     constexpr int G4 = 128 / BLK, RT = 16 * MT, GUARDA = ilog2_c(BLK) - 4;
     extern __shared__ float lds[];
@@ -44,86 +49,112 @@ __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) k_gemv4(gv4::Args a) {
     float* rs = lds;                                                  // [nb][MT][4: m % 4][4: m / 4]
     int* RA = reinterpret_cast<int*>(rs + nb * RT);                   // [RT]
     int* soma = RA + RT;                                              // [RT][cols]
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, c = lane >> 4, n = lane & 15;
+    constexpr int XS = 144;                                           // bytes of an X row's 128 in a wave's own piece of LDS
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, c = lane >> 4, n = lane & 15;
     const int ks = w % a.KS, cg = w / a.KS, m0 = blockIdx.y * RT;
+    int8_t* xl = reinterpret_cast<int8_t*>(soma + RT * cols) + w * RT * XS;
     const int nt0 = (blockIdx.x * a.CG + cg) * CT;
 
-    int4 W[CT];
-    uint2 S[CT];
-    int2 X[MT][4];
-    auto carrega = [&](int kt) {
+    // the exponents of the wave's first row of X, then its first steps' bytes: waiting for the exponents leaves those in flight
+    int ex[4];
+    const int8_t* e0 = a.xE + (long long)min(m0 + w, a.M - 1) * nb;
+#pragma unroll
+    for (int k = 0; k < 4; k++) ex[k] = e0[min(lane + 64 * k, nb - 1)];
+    constexpr int D = 2;                                              // steps whose weights are in flight
+    int4 W[D][CT];
+    uint2 S[D][CT];
+    v4i X[MT][2];                                                     // X's bytes of the next step: 16 a lane, 8 lanes a row, whole lines
+    unsigned linha[MT][2];
+#pragma unroll
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) linha[t][k] = (unsigned)(min(m0 + 16 * t + 8 * k + lane / 8, a.M - 1) - min(m0, a.M - 1)) * a.K;
+    const int8_t* x0 = a.x + (long long)min(m0, a.M - 1) * a.K;
+    auto carrega_w = [&](int z, int kt) {
 #pragma unroll
         for (int t = 0; t < CT; t++) {
             const long long tile = (long long)min(nt0 + t, Nt - 1) * Kt + kt;
-            W[t] = a.w[tile * 64 + lane];
-            if constexpr (G4 == 4) S[t] = *reinterpret_cast<const uint2*>(a.esc + (tile * 16 + n) * 4);
-            else S[t].x = a.esc[tile * 16 + n];
-        }
-#pragma unroll
-        for (int t = 0; t < MT; t++) {
-            const int8_t* x = a.x + (long long)min(m0 + 16 * t + n / 4 + 4 * (n % 4), a.M - 1) * a.K + 8 * c;
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int k = 128 * kt + 32 * q;
-                X[t][q] = *reinterpret_cast<const int2*>(x + (k < a.K ? k : 0));       // past K the weights are zeros
-            }
+            W[z][t] = (a.w + tile * 64)[lane];
+            const uint16_t* s = a.esc + tile * 16 * G4;
+            if constexpr (G4 == 4) S[z][t] = reinterpret_cast<const uint2*>(s)[n];
+            else S[z][t].x = s[n];
         }
     };
-    carrega(min(ks, Kt - 1));
+    auto carrega_x = [&](int kt) {
+        const int k = 128 * kt + 16 * (lane % 8), o = k < a.K ? k : 0;                 // past K the weights are zeros
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) X[t][i] = *reinterpret_cast<const v4i*>(x0 + linha[t][i] + o);
+    };
+    carrega_x(min(ks, Kt - 1));
+#pragma unroll
+    for (int z = 0; z < D; z++) carrega_w(z, min(ks + z * a.KS, Kt - 1));
 
     for (int m = w; m < RT; m += nw) {                                // exponents of X's rows, as scales of each block
-        const int8_t* e = a.xE + (long long)min(m0 + m, a.M - 1) * nb;
-        int mx = -128;
-        for (int b = lane; b < nb; b += 64) mx = max(mx, (int)e[b]);
-        mx = g_max<64>(mx);
+        if (m > w) {
+            const int8_t* e = a.xE + (long long)min(m0 + m, a.M - 1) * nb;
+#pragma unroll
+            for (int k = 0; k < 4; k++) ex[k] = e[min(lane + 64 * k, nb - 1)];
+        }
+        const int mx = g_max<64>(max(max(ex[0], ex[1]), max(ex[2], ex[3])));
         if (lane == 0) RA[m] = mx;
-        for (int b = lane; b < nb; b += 64) rs[b * RT + (m & ~15) + 4 * (m % 4) + (m / 4) % 4] = __builtin_ldexpf(1.f, e[b] - mx - GUARDA - 4);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (lane + 64 * k < nb) rs[(lane + 64 * k) * RT + (m & ~15) + 4 * (m % 4) + (m / 4) % 4] = __builtin_ldexpf(1.f, ex[k] - mx - GUARDA - 4);
     }
     for (int k = threadIdx.x; k < RT * cols; k += blockDim.x) soma[k] = 0;
     __syncthreads();
 
     int acc[CT][MT][NR] = {}, conta = 0;
-    for (int kt = ks; kt < Kt; kt += a.KS) {
-        int4 Wc[CT];
-        uint2 Sc[CT];
-        int2 Xc[MT][4];
-#pragma unroll
-        for (int t = 0; t < CT; t++) { Wc[t] = W[t]; Sc[t] = S[t]; }
+    auto guarda_x = [&] {                                             // row m of 16 goes to slot 4 (m % 4) + m / 4
 #pragma unroll
         for (int t = 0; t < MT; t++)
 #pragma unroll
-            for (int q = 0; q < 4; q++) Xc[t][q] = X[t][q];
-        carrega(min(kt + a.KS, Kt - 1));
+            for (int i = 0; i < 2; i++) {
+                const int m = 8 * i + lane / 8;
+                *reinterpret_cast<v4i*>(xl + (16 * t + 4 * (m % 4) + m / 4) * XS + 16 * (lane % 8)) = X[t][i];
+            }
+    };
+    auto usa = [&](int z, int kt) {
         v4i p[CT][MT];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            if (128 * kt + 32 * q >= a.K) break;
-            const int b = (128 * kt + 32 * q) / BLK;
+            const int b = min((128 * kt + 32 * q) / BLK, nb - 1);     // past K the weights are zeros: 0 is added, without a branch
+            long wq[CT];
 #pragma unroll
             for (int t = 0; t < CT; t++) {
-                const int x = q == 0 ? Wc[t].x : q == 1 ? Wc[t].y : q == 2 ? Wc[t].z : Wc[t].w;
-                const long wq = (long)(((unsigned long)(unsigned)(x & 0xF0F0F0F0) << 32) | (unsigned)((x << 4) & 0xF0F0F0F0));
-#pragma unroll
-                for (int u = 0; u < MT; u++) {
-                    const long xq = (long)(((unsigned long)(unsigned)Xc[u][q].y << 32) | (unsigned)Xc[u][q].x);
-                    p[t][u] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xq, wq, BLK == 32 || q == 0 ? v4i{0, 0, 0, 0} : p[t][u], 0, 0, 0);
-                }
+                const int x = q == 0 ? W[z][t].x : q == 1 ? W[z][t].y : q == 2 ? W[z][t].z : W[z][t].w;
+                wq[t] = (long)(((unsigned long)(unsigned)(x & 0xF0F0F0F0) << 32) | (unsigned)((x << 4) & 0xF0F0F0F0));
             }
-            if (BLK == 128 && q < 3) continue;
-            conta++;
 #pragma unroll
             for (int u = 0; u < MT; u++) {
-                float r[NR];
+                const long xq = __builtin_bit_cast(long, *reinterpret_cast<const v2i*>(xl + (16 * u + n) * XS + 32 * q + 8 * c));
 #pragma unroll
-                for (int k = 0; k < NR; k++) r[k] = rs[b * RT + 16 * u + 4 * c + k];
+                for (int t = 0; t < CT; t++) p[t][u] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xq, wq[t], BLK == 32 || q == 0 ? v4i{0, 0, 0, 0} : p[t][u], 0, 0, 0);
+                if (BLK == 128 && q < 3) continue;
+                const v4i r = *reinterpret_cast<const v4i*>(rs + b * RT + 16 * u + 4 * c);
 #pragma unroll
                 for (int t = 0; t < CT; t++) {
-                    const unsigned s = (q & 2) && BLK == 32 ? Sc[t].y : Sc[t].x;
+                    const unsigned s = (q & 2) && BLK == 32 ? S[z][t].y : S[z][t].x;
                     const float sc = __int_as_float(BLK == 32 && (q & 1) ? s & 0xffff0000u : s << 16);
 #pragma unroll
-                    for (int k = 0; k < NR; k++)
-                        acc[t][u][k] += __float_as_int(__builtin_fmaf((float)p[t][u][k], sc * r[k], 12582912.f));
+                    for (int k = 0; k < NR; k++) acc[t][u][k] += __float_as_int(__builtin_fmaf((float)p[t][u][k], sc * __int_as_float(r[k]), 12582912.f));
+                    if constexpr (NR < 4) asm volatile("" ::"v"(p[t][u]));             // keeps the unread registers of a product from other products
                 }
+            }
+        }
+        conta += 128 / BLK;
+    };
+    for (int kt = ks; kt < Kt; kt += D * a.KS) {
+#pragma unroll
+        for (int z = 0; z < D; z++) {
+            const int k = kt + z * a.KS;
+            if (k < Kt) {
+                guarda_x();
+                carrega_x(min(k + a.KS, Kt - 1));
+                usa(z, k);
+                carrega_w(z, min(k + D * a.KS, Kt - 1));
             }
         }
     }
