@@ -1009,7 +1009,7 @@ int jt_cache_grava(const void* qm, const void* qE, void* cm, void* cE, int npag,
     const atc::Lote L{(const int*)tab, (const int*)comp, (const int*)ini, B, P, M, ilog2(pag), npag, novos, teto};
     const long long camada_m = 2LL * Hk * pag * hd, camada_e = 2LL * Hk * pag * grupos(hd);
     const int rpw = hd <= 16 ? 64 : 1024 / hd;                        // rows per wave
-    const dim3 grade((M + rpw - 1) / rpw, (2 * Hk + 3) / 4);
+    const dim3 grade((M - 1) / rpw + 2u, (2 * Hk + 3) / 4);           // the last column of workgroups checks the sequences
 #define F(HD, GS) (k_cache_grava<HD, GS><<<grade, 256, 0, g_stream>>>((const int8_t*)qm, (const int8_t*)qE, (int8_t*)cm + camada * camada_m, \
                    (int8_t*)cE + camada * camada_e, L, H, Hk, ilog2(g_blk), camadas * camada_m, camadas * camada_e, kid))
     POR_CABECA(F)
@@ -1098,7 +1098,7 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
                       tipo != 0 || hd >= g_blk, H, Hk, ilog2(g_blk), janela, sumid, p.S, p.fatia, tipo, kid};
 #define F(HD, GS) (p.tipo == ATC_MF ? k_atc_mf<HD, GS><<<dim3(p.tiles, Hk, p.S), 256, 0, g_stream>>>(a) \
                    : p.tipo == ATC_GR ? k_atc_gr<HD, GS><<<dim3(B + 1, Hk, p.S), 256, 0, g_stream>>>(a) \
-                                      : k_atc_um<HD, GS><<<dim3(M, H, p.S), 256, 0, g_stream>>>(a))
+                                      : k_atc_um<HD, GS><<<dim3(M + 1u, H, p.S), 256, 0, g_stream>>>(a))
     POR_CABECA(F)
 #undef F
     int rc = fim();

@@ -20,14 +20,20 @@ struct Lote {
     int B, P, M, lgpag, npag, novos, teto;       // novos: most rows of a sequence; teto: most tokens
 };
 
-// first row, row count and length of sequence b; false (and E_ARG, from the one lane that asks) where they are malformed
-__device__ __forceinline__ bool sequencia(const Lote& L, int b, int& r0, int& n, int& comp, int kid, bool relata) {
+// first row, row count and length of sequence b; false where they are malformed
+__device__ __forceinline__ bool sequencia(const Lote& L, int b, int& r0, int& n, int& comp) {
     comp = L.comp[b];
     r0 = L.ini ? L.ini[b] : b;
     n = L.ini ? L.ini[b + 1] - r0 : min(comp, 1);                     // without starts, an empty sequence has no row
-    const bool ok = r0 >= 0 && n >= 0 && r0 <= L.M - n && n <= L.novos && comp >= n && comp <= L.teto;
-    if (!ok && relata) reporta(E_ARG, kid, r0, comp, b);
-    return ok;
+    return r0 >= 0 && n >= 0 && r0 <= L.M - n && n <= L.novos && comp >= n && comp <= L.teto;
+}
+
+// E_ARG for every malformed sequence, by one workgroup of a launch: a sequence that nobody comes upon by a row of its own (starts that
+// fall back) is found here
+__device__ __forceinline__ void confere(const Lote& L, int kid) {
+    int r0, n, comp;
+    for (int b = threadIdx.x; b < L.B; b += blockDim.x)
+        if (!sequencia(L, b, r0, n, comp)) reporta(E_ARG, kid, r0, comp, b);
 }
 
 // The sequence of row r, found by a whole wave: every lane looks at one of 64 starts, and the last start at or below r
@@ -43,7 +49,7 @@ __device__ __forceinline__ int sequencia_de(const Lote& L, int r) {
 }
 
 // the same with the sequence's own numbers, which the lanes load beside the starts: still one round trip
-__device__ __forceinline__ Seq acha(const Lote& L, int r, int kid, bool relata) {
+__device__ __forceinline__ Seq acha(const Lote& L, int r) {
     Seq s{-1, 0, 0};
     int r0 = r, fim = r + 1, comp = 0;
     if (L.ini) {
@@ -66,7 +72,6 @@ __device__ __forceinline__ Seq acha(const Lote& L, int r, int kid, bool relata) 
     if (s.b < 0) return s;
     const int n = fim - r0;
     s.ok = r0 >= 0 && n >= 0 && r0 <= L.M - n && n <= L.novos && comp >= n && comp <= L.teto;
-    if (!s.ok && relata) reporta(E_ARG, kid, r0, comp, s.b);
     s.ok = s.ok && r - r0 < n;
     s.i = comp - n + (r - r0);
     return s;
@@ -85,6 +90,10 @@ __global__ void __launch_bounds__(256) k_cache_grava(const int8_t* __restrict__ 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int r = blockIdx.x * LPW + lane / NC, c = lane % NC;
     const int kvh = blockIdx.y * 4 + w;                                                 // keys' heads, then values'
+    if (blockIdx.x == gridDim.x - 1) {                                                  // has no rows
+        if (blockIdx.y == 0) atc::confere(L, kid);
+        return;
+    }
     if (kvh >= 2 * Hk) return;
     // one search per wave for its first row; the rows after it follow
     int b = atc::sequencia_de(L, min((int)(blockIdx.x * LPW), L.M - 1));
@@ -95,7 +104,7 @@ __global__ void __launch_bounds__(256) k_cache_grava(const int8_t* __restrict__ 
         if (b >= L.B || r < L.ini[b]) return;                                           // behind the last sequence
     } else if ((b = r) >= L.B) return;
     int r0, n, comp;
-    if (!atc::sequencia(L, b, r0, n, comp, kid, kvh == 0 && c == 0) || r - r0 >= n) return;
+    if (!atc::sequencia(L, b, r0, n, comp) || r - r0 >= n) return;
     const int j = comp - n + (r - r0), pag = 1 << L.lgpag;
     const int p = L.tab[(long long)b * L.P + (j >> L.lgpag)];
     if ((unsigned)p >= (unsigned)L.npag) {
@@ -223,7 +232,7 @@ __global__ void __launch_bounds__(NG == 2 ? 256 : 32 * NG) k_atc_junta(const flo
     const int r = blockIdx.x, ct = threadIdx.x & 31, g = (threadIdx.x >> 5) % NG, faixa = NG == 2 ? blockIdx.y * 4 + (threadIdx.x >> 6) : blockIdx.y;
     const int col = faixa * 128 + 4 * ct, cc = min(col, C - 4);
     const long long part = ((long long)r * (C / hd) + cc / hd) * S;
-    const bool escrita = ml[2 * part] == INFINITY || col >= C;        // by its one split
+    const bool escrita = ml[2 * part + 1] < 0.f || col >= C;          // by its one split
     if (__all(escrita)) return;                                       // the waves that share splits have the same columns
     float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = g; s0 < S; s0 += 4 * NG) {
@@ -235,7 +244,7 @@ __global__ void __launch_bounds__(NG == 2 ? 256 : 32 * NG) k_atc_junta(const flo
             const int s = s0 + k * NG;
             x[k] = *reinterpret_cast<const float2*>(ml + 2 * (part + min(s, S - 1)));
             y[k] = *reinterpret_cast<const float4*>(po + (part + min(s, S - 1)) * hd + cc % hd);
-            x[k].x = s < S && x[k].x != INFINITY ? x[k].x : -INFINITY;
+            x[k].x = s < S ? x[k].x : -INFINITY;
             mn = fmaxf(mn, x[k].x);
         }
         const float al = atc::fator(M, mn);
@@ -246,7 +255,7 @@ __global__ void __launch_bounds__(NG == 2 ? 256 : 32 * NG) k_atc_junta(const flo
 #pragma unroll
         for (int k = 0; k < 4; k++) {                                 // a split without tokens has left its outputs unwritten
             const float f = atc::fator(x[k].x, M);
-            const bool tem = f > 0.f;
+            const bool tem = f != 0.f || x[k].y != x[k].y;            // scores beyond fp32: f or the sum is NaN
             L += tem ? f * x[k].y : 0.f;
             v[0] += tem ? f * y[k].x : 0.f; v[1] += tem ? f * y[k].y : 0.f;
             v[2] += tem ? f * y[k].z : 0.f; v[3] += tem ? f * y[k].w : 0.f;
@@ -350,7 +359,7 @@ __device__ __forceinline__ bool linhas_de(const Args& a, int b, bool primeiro, i
         for (long long x = max(fim, 0) + (long long)parte; x < a.L.M; x += passo) vazia<HD>(a, x, hk);
         return false;
     }
-    if (!sequencia(a.L, b, r0, n, comp, a.kid, primeiro && threadIdx.x == 0 && hk == 0 && blockIdx.z == 0)) {
+    if (!sequencia(a.L, b, r0, n, comp)) {
         const long long fim = a.L.ini ? (long long)a.L.ini[b + 1] : b + 1;
         if (primeiro)
             for (long long r = max(r0, 0); r < min(fim, (long long)a.L.M); r++) vazia<HD>(a, r, hk);
@@ -428,8 +437,8 @@ struct Linha {
             i4_t p = {0, 0, 0, 0};
 #pragma unroll
             for (int k = g * MPG; k < (g + 1) * MPG; k++) p = __builtin_amdgcn_mfma_i32_16x16x32_i8(kf[k], q[k], p, 0, 0, 0);
-            x[0] += (float)p[0] * f[g].x * fq[g]; x[1] += (float)p[1] * f[g].y * fq[g];
-            x[2] += (float)p[2] * f[g].z * fq[g]; x[3] += (float)p[3] * f[g].w * fq[g];
+            x[0] += (float)p[0] * (f[g].x * fq[g]); x[1] += (float)p[1] * (f[g].y * fq[g]);
+            x[2] += (float)p[2] * (f[g].z * fq[g]); x[3] += (float)p[3] * (f[g].w * fq[g]);
         }
 #pragma unroll
         for (int k = 0; k < 4; k++) s[k] = __builtin_fmaf(-incl, (float)(i - j) - (float)k, x[k]);   // distances below 2^24 are exact
@@ -484,14 +493,14 @@ struct Corrente {
         l += __shfl_xor(l, 32);
     }
     // the row's output, or its partial result. `uma`: this split is the row's only one; where blocks lie in a head the output is
-    // then written here, and an infinite maximum tells the join so.
+    // then written here, and a negative sum tells the join so.
     template <int GS>
     __device__ __forceinline__ void grava(const Args& a, long long r, int h, int c, bool uma) {
         const int C = a.H * HD;
         const long long part = (r * a.H + h) * a.S + blockIdx.z;
         if (a.ml && uma && a.inteira) {
             if (blockIdx.z > 0) return;
-            if (c == 0) a.ml[2 * part] = INFINITY;
+            if (c == 0) a.ml[2 * part + 1] = -1.f;
         } else if (a.ml) {
             if (c == 0) { a.ml[2 * part] = m; a.ml[2 * part + 1] = l; }
             if (HD >= 16 || c == 0)
@@ -586,7 +595,8 @@ __device__ __forceinline__ int4 le_vb(const int8_t* p) {
 // and they are joined at the end (lanes, waves, then the splits by k_atc_junta). Products of mantissas are exact in int32
 // (v_dot4), statistics and outputs fp32. Only the page table is read a tile ahead: holding the next tile's bytes too costs a fifth
 // of the waves and is slower (104 us against 92 below).
-// Reading the keys and values bounds it: 4 sequences of 90,001 to 131,071 tokens, 8 heads of 64.
+// Reading the keys and values bounds it: 4 sequences of 90,001 to 131,071 tokens, 8 heads of 64 take 94 us, 4.97 TB/s of cache (a
+// large copy reaches 5.5). Short contexts are latency: one of 200 tokens 6.7 us, the launch and three round trips to memory.
 template <int HD, int GS>
 __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
     using namespace atc;
@@ -594,7 +604,11 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
     constexpr bool UMA = KPW <= 16;                                   // a wave load's keys lie in one page
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane % LPK;
     const int r = blockIdx.x, h = blockIdx.y, hk = h / (a.H / a.Hk), g = c * VB / GS, pag = 1 << a.L.lgpag;
-    const Seq q = acha(a.L, r, a.kid, threadIdx.x == 0 && h == 0 && blockIdx.z == 0);
+    if (r == a.L.M) {                                                 // past the rows
+        if (h == 0 && blockIdx.z == 0) confere(a.L, a.kid);
+        return;
+    }
+    const Seq q = acha(a.L, r);
     Tiles<TK> tl(a, max(q.i, 0), max(q.i, 0));
     if (!q.ok) { tl.t0 = tl.t1 = 0; tl.uma = true; }
 
@@ -739,7 +753,7 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
     }
     if (a.ml) {                                                       // the row's one split: written here
         if (blockIdx.z > 0) return;
-        if (threadIdx.x == 0) a.ml[2 * part] = INFINITY;
+        if (threadIdx.x == 0) a.ml[2 * part + 1] = -1.f;
     }
     const float inv = LL == 0.f ? 0.f : 1.f / LL;
 #pragma unroll
@@ -767,6 +781,7 @@ __global__ void __launch_bounds__(256) k_atc_mf(atc::Args a) {
     constexpr int NT = TK * LPK, IT = (NT + 255) / 256; // staging: chunks of a tile's keys (and of its values), per thread
     __shared__ __align__(16) __bf16 sk[2][TK * VS], sv[2][TK * VS];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk;
+    if (blockIdx.x == gridDim.x - 1 && hk == 0 && blockIdx.z == 0) confere(a.L, a.kid);
     int b, tile = 0, total, r0, n, comp;
     tile_de(a, blockIdx.x, RW, b, tile, total);
     if (!linhas_de<HD>(a, b, tile == 0, blockIdx.x - total, gridDim.x - total, hk, r0, n, comp)) return;
@@ -900,6 +915,7 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk;
     __bf16* sv = reinterpret_cast<__bf16*>(mem + w * (BV + BF));
     float* sf = reinterpret_cast<float*>(mem + w * (BV + BF) + BV);
+    if (blockIdx.x == gridDim.x - 1 && hk == 0 && blockIdx.z == 0) confere(a.L, a.kid);
     int r0, n, comp;
     if (!linhas_de<HD>(a, blockIdx.x, true, 0, 1, hk, r0, n, comp)) return;
     const int b = blockIdx.x, linhas = n * Gq, i_lo = comp - n, i_hi = comp - 1, pag = 1 << a.L.lgpag;
