@@ -99,6 +99,8 @@ class OpsHip:
     def _a(x):
         """x as a C argument: a tensor's address (0 when it is empty), a null pointer for None, and an int that fits
         32 bits as it is, which ctypes passes as a C int."""
+        if type(x) is int:
+            return x if -2**31 < x < 2**31 else ctypes.c_longlong(x)
         if isinstance(x, torch.Tensor):
             return ctypes.c_void_p(x.data_ptr())
         if x is None:
