@@ -1098,7 +1098,7 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
                       tipo != 0 || hd >= g_blk, H, Hk, ilog2(g_blk), janela, sumid, p.S, p.fatia, tipo, kid};
 #define F(HD, GS) (p.tipo == ATC_MF ? k_atc_mf<HD, GS><<<dim3(p.tiles, Hk, p.S), 256, 0, g_stream>>>(a) \
                    : p.tipo == ATC_GR ? k_atc_gr<HD, GS><<<dim3(B + 1, Hk, p.S), 256, 0, g_stream>>>(a) \
-                                      : k_atc_um<HD, GS><<<dim3(M + 1u, H, p.S), 256, 0, g_stream>>>(a))
+                                      : k_atc_um<HD, GS><<<dim3(M, H, p.S), 256, 0, g_stream>>>(a))
     POR_CABECA(F)
 #undef F
     int rc = fim();

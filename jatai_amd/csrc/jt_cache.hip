@@ -30,9 +30,9 @@ __device__ __forceinline__ bool sequencia(const Lote& L, int b, int& r0, int& n,
 
 // E_ARG for every malformed sequence, by one workgroup of a launch: a sequence that nobody comes upon by a row of its own (starts that
 // fall back) is found here
-__device__ __forceinline__ void confere(const Lote& L, int kid) {
+__device__ __forceinline__ void confere(const Lote& L, int kid, int parte, int passo) {
     int r0, n, comp;
-    for (int b = threadIdx.x; b < L.B; b += blockDim.x)
+    for (int b = parte; b < L.B; b += passo)
         if (!sequencia(L, b, r0, n, comp)) reporta(E_ARG, kid, r0, comp, b);
 }
 
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256) k_cache_grava(const int8_t* __restrict__ 
     const int r = blockIdx.x * LPW + lane / NC, c = lane % NC;
     const int kvh = blockIdx.y * 4 + w;                                                 // keys' heads, then values'
     if (blockIdx.x == gridDim.x - 1) {                                                  // has no rows
-        if (blockIdx.y == 0) atc::confere(L, kid);
+        if (blockIdx.y == 0) atc::confere(L, kid, threadIdx.x, 256);
         return;
     }
     if (kvh >= 2 * Hk) return;
@@ -604,10 +604,6 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
     constexpr bool UMA = KPW <= 16;                                   // a wave load's keys lie in one page
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane % LPK;
     const int r = blockIdx.x, h = blockIdx.y, hk = h / (a.H / a.Hk), g = c * VB / GS, pag = 1 << a.L.lgpag;
-    if (r == a.L.M) {                                                 // past the rows
-        if (h == 0 && blockIdx.z == 0) confere(a.L, a.kid);
-        return;
-    }
     const Seq q = acha(a.L, r);
     Tiles<TK> tl(a, max(q.i, 0), max(q.i, 0));
     if (!q.ok) { tl.t0 = tl.t1 = 0; tl.uma = true; }
@@ -734,7 +730,10 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
     for (int d = 0; d < RESTO; d++) so[w][c * VB + d0 + d] = o[d];    // lanes with the same values write the same
     if (lane == 0) { sm[w] = M; sl[w] = l; }
     __syncthreads();
-    if (threadIdx.x >= HD / 4) return;
+    if (threadIdx.x >= HD / 4) {
+        if (r == 0 && h == 0 && blockIdx.z == 0) confere(a.L, a.kid, threadIdx.x - HD / 4, 256 - HD / 4);
+        return;
+    }
     float MM = sm[0], LL = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 1; k < NW; k++) MM = fmaxf(MM, sm[k]);
@@ -781,7 +780,7 @@ __global__ void __launch_bounds__(256) k_atc_mf(atc::Args a) {
     constexpr int NT = TK * LPK, IT = (NT + 255) / 256; // staging: chunks of a tile's keys (and of its values), per thread
     __shared__ __align__(16) __bf16 sk[2][TK * VS], sv[2][TK * VS];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk;
-    if (blockIdx.x == gridDim.x - 1 && hk == 0 && blockIdx.z == 0) confere(a.L, a.kid);
+    if (blockIdx.x == gridDim.x - 1 && hk == 0 && blockIdx.z == 0) confere(a.L, a.kid, threadIdx.x, 256);
     int b, tile = 0, total, r0, n, comp;
     tile_de(a, blockIdx.x, RW, b, tile, total);
     if (!linhas_de<HD>(a, b, tile == 0, blockIdx.x - total, gridDim.x - total, hk, r0, n, comp)) return;
@@ -915,7 +914,7 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4, hk = blockIdx.y, Gq = a.H / a.Hk;
     __bf16* sv = reinterpret_cast<__bf16*>(mem + w * (BV + BF));
     float* sf = reinterpret_cast<float*>(mem + w * (BV + BF) + BV);
-    if (blockIdx.x == gridDim.x - 1 && hk == 0 && blockIdx.z == 0) confere(a.L, a.kid);
+    if (blockIdx.x == gridDim.x - 1 && hk == 0 && blockIdx.z == 0) confere(a.L, a.kid, threadIdx.x, 256);
     int r0, n, comp;
     if (!linhas_de<HD>(a, blockIdx.x, true, 0, 1, hk, r0, n, comp)) return;
     const int b = blockIdx.x, linhas = n * Gq, i_lo = comp - n, i_hi = comp - 1, pag = 1 << a.L.lgpag;

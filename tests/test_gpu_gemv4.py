@@ -136,3 +136,57 @@ def test_gemv4_fundido(blk, M, N, K):
     for y, z in ((g.ops.gemv4(X, P), h), (g.ops.gemv4_soma(X, P, res), g.ops.soma(res, h)), (g.ops.gemv4_relu2(X, P), g.ops.relu2(h))):
         assert torch.equal(y[0], z[0]) and torch.equal(y[1], z[1])
     g.reg.fim_passo()
+
+
+def test_pesos_alem_de_2_gib():
+    """The last rows of weights whose packed bytes pass 2^31 (and whose mantissas pass 2^32): packed and multiplied as by themselves."""
+    N, K, blk, n = 270000, 16384, 128, 64
+    m, E = _pesos(9, n, K, blk)
+    xm, xE = R.bloco(10, 3, K, blk, espalha=6, e0=-4)
+    g = GPU(blk)
+    W = torch.zeros(N, K, dtype=torch.int8, device="cuda"), torch.full((N, K // blk), -127, dtype=torch.int8, device="cuda")
+    for d, x in zip(W, (m, E)):
+        d[-n:] = g.dev(x)
+    P, p = g.ops.para4(W), g.ops.para4((g.dev(m), g.dev(E)))
+    assert P[0].numel() > 2**31 and all(torch.equal(a[-b.shape[0]:], b) for a, b in zip(P, p))
+    X = g.dev(xm), g.dev(xE)
+    (acc, e), (a, ee) = g.ops.gemv4(X, P, cru=True), g.ops.gemv4(X, p, cru=True)
+    g.reg.fim_passo()
+    assert torch.equal(acc[:, -n:], a) and torch.equal(e[:, -n:], ee) and not acc[:, :-n].any() and bool(a.any())
+
+
+def test_gemv4_sem_linhas_gravado_e_noutra_corrente():
+    blk, N, K = 32, 256, 640
+    g = GPU(blk)
+    P = g.ops.para4(tuple(map(g.dev, _pesos(11, N, K, blk))))
+    z = g.ops.gemv4((torch.zeros(0, K, dtype=torch.int8, device="cuda"), torch.zeros(0, K // blk, dtype=torch.int8, device="cuda")), P)
+    assert z[0].shape == (0, N) and z[1].shape == (0, N // blk)
+    entradas = [tuple(map(g.dev, R.bloco(R.substream(12, f"{k}"), 5, K, blk, espalha=6, e0=-4))) for k in range(3)]
+    res = tuple(map(g.dev, R.bloco(13, 5, N, blk, e0=-6)))
+    certas = [g.ops.valores(g.ops.gemv4_soma(X, P, res)) for X in entradas]
+    X = tuple(t.clone() for t in entradas[0])
+    torch.cuda.synchronize()
+    grafo = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(grafo):
+            g.ops.lib.jt_stream(torch.cuda.current_stream().cuda_stream)
+            y = g.ops.valores(g.ops.gemv4_soma(X, P, res))
+    finally:
+        g.ops.lib.jt_stream(None)
+    for novo, certa in list(zip(entradas, certas)) * 2:
+        for d, o in zip(X, novo):
+            d.copy_(o)
+        grafo.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, certa) and torch.equal(g.ops.valores(g.ops.gemv4_soma(novo, P, res)), certa)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g.ops.lib.jt_stream(s.cuda_stream)
+        try:
+            y = g.ops.valores(g.ops.gemv4_soma(tuple(t.clone() for t in entradas[1]), P, res)) + 0
+        finally:
+            g.ops.lib.jt_stream(None)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y, certas[1])
+    g.reg.fim_passo()
