@@ -1104,8 +1104,10 @@ int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void*
     int rc = fim();
     if (rc || p.direto) return rc;
     const int C = H * hd;
-    const dim3 grade(M, p.S <= 8 ? (C + 511) / 512 : (C + 127) / 128);
-#define J(BL, T) (p.S <= 8 ? k_atc_junta<BL, T, 2><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)       \
+    const int wg1 = 64 * std::min(4, (C + 255) / 256);
+    const dim3 grade(M, p.S <= 4 ? (C + 4 * wg1 - 1) / (4 * wg1) : p.S <= 8 ? (C + 511) / 512 : (C + 127) / 128);
+#define J(BL, T) (p.S <= 4 ? k_atc_junta<BL, T, 1><<<grade, wg1, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)       \
+                  : p.S <= 8 ? k_atc_junta<BL, T, 2><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)       \
                   : p.S <= 32 ? k_atc_junta<BL, T, 8><<<grade, 256, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid)   \
                               : k_atc_junta<BL, T, 32><<<grade, 1024, 0, g_stream>>>(ml, po, out, (int8_t*)outE, C, hd, p.S, kid))
     if (tipo == 1) J(32, 1);

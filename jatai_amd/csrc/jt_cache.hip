@@ -225,12 +225,14 @@ __device__ __forceinline__ void grava_4(void* out, int8_t* outE, int tipo, long 
 // Joins the splits of a row and head, o = sum exp(m_s - m) o_s / sum exp(m_s - m) l_s (zeros for a row without visible
 // tokens), and writes the row as a block tensor (TIPO 0), bfloat16 (1) or fp32 (2). NG groups of 32 threads share out the splits
 // of 128 columns of a row, 4 columns a thread, four splits in flight at a time: one thread walking 64 splits one by one
-// waited for each (30 us of a call of 131). With NG = 2 the groups are one wave, and a workgroup takes 512 columns in four of them.
+// waited for each (30 us of a call of 131). With NG = 2 the groups are one wave, and a workgroup takes 512 columns in four of them;
+// up to four splits (NG = 1) a wave takes 256 columns alone, there being nothing to share out.
 template <int BLK, int TIPO, int NG>
-__global__ void __launch_bounds__(NG == 2 ? 256 : 32 * NG) k_atc_junta(const float* __restrict__ ml, const float* __restrict__ po, void* __restrict__ out,
+__global__ void __launch_bounds__(NG <= 2 ? 256 : 32 * NG) k_atc_junta(const float* __restrict__ ml, const float* __restrict__ po, void* __restrict__ out,
                                                                        int8_t* __restrict__ oE, int C, int hd, int S, int kid) {
-    const int r = blockIdx.x, ct = threadIdx.x & 31, g = (threadIdx.x >> 5) % NG, faixa = NG == 2 ? blockIdx.y * 4 + (threadIdx.x >> 6) : blockIdx.y;
-    const int col = faixa * 128 + 4 * ct, cc = min(col, C - 4);
+    constexpr int LC = NG == 1 ? 64 : 32;                             // lanes side by side along the columns
+    const int r = blockIdx.x, ct = threadIdx.x % LC, g = threadIdx.x / LC % NG, faixa = NG <= 2 ? blockIdx.y * (blockDim.x >> 6) + (threadIdx.x >> 6) : blockIdx.y;
+    const int col = faixa * 4 * LC + 4 * ct, cc = min(col, C - 4);
     const long long part = ((long long)r * (C / hd) + cc / hd) * S;
     const bool escrita = ml[2 * part + 1] < 0.f || col >= C;          // by its one split
     if (__all(escrita)) return;                                       // the waves that share splits have the same columns
@@ -261,7 +263,9 @@ __global__ void __launch_bounds__(NG == 2 ? 256 : 32 * NG) k_atc_junta(const flo
             v[2] += tem ? f * y[k].z : 0.f; v[3] += tem ? f * y[k].w : 0.f;
         }
     }
-    if constexpr (NG == 2) {
+    if constexpr (NG == 1) {
+        if (escrita) return;
+    } else if constexpr (NG == 2) {
         const float MM = fmaxf(M, __shfl_xor(M, 32)), f = atc::fator(M, MM);
         L = L * f + __shfl_xor(L * f, 32);
 #pragma unroll
