@@ -767,7 +767,8 @@ class OpsHip:
         the tokens j <= i of its sequence; with janela > 0 the last `janela` of them and the first `sumidouros`:
             softmax_j(q . k_j / sqrt(hd) - incl[h] (i - j)) . v_j,  incl float32 [H] or None (see inclinacoes)
         Products are exact, statistics float32. Returns a block tensor [M, H hd] (saida None) or a torch.bfloat16 or
-        torch.float32 tensor, rounded once; rows that belong to no sequence come out as zeros."""
+        torch.float32 tensor, rounded once; rows that belong to no sequence come out as zeros. Scores beyond float32 give NaN,
+        or an exponent event in a block tensor."""
         paginas, camadas, Hk, hd, pag, H, B, P = self._confere_lote("atencao_cache", QKV, C, camada, lote)
         m, E = QKV
         M, D = m.shape[0], H * hd
