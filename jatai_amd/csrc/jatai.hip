@@ -1052,7 +1052,8 @@ int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, in
 // number two per CU, with at least one tile a wave (um) or two (gr): a row's work is all reading, and every workgroup more costs
 // its start, its end and its part of the join (long contexts above at 512, 1024, 2048 workgroups 94, 101, 99 us; 64 sequences in a
 // window of 1024 19, 25, 27). Rows of prompts, 1024 workgroups, at least four tiles each and at most 24, so that the longest row
-// does not outlast the others (8 prompts of up to 4000 tokens at 12, 24, 40 tiles and undivided: 208, 190, 200 and 239 us).
+// does not outlast the others (8 prompts of up to 4000 tokens at 24 and 32 tiles 187 and 193 us; with three waves a SIMD at 12, 24, 40 and undivided
+// 208, 190, 200 and 239).
 // direto: one split, and every block of the output lies in a head, so the kernel writes it and there is no join.
 enum { ATC_UM, ATC_GR, ATC_MF };
 struct PlanoAtc { int tipo; bool direto; unsigned tiles; int S, fatia; };

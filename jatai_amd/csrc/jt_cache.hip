@@ -81,7 +81,8 @@ __device__ __forceinline__ Seq acha(const Lote& L, int r) {
 // ---------------------------------------------------------------------------------------------- pages
 // The rows' keys and values into their slots. A thread moves VB bytes (a head's 16, or its 4): the threads of a wave hold
 // the same chunks of consecutive rows, whose slots are consecutive, so a wave writes whole kilobytes of a page's tile.
-// Bound by its bytes, read and written once.
+// Bound by its bytes, read and written once: 16 prompts of 300 to 2048 tokens, 8 heads of 64, 10.9 us (3.7 TB/s, the launch's start and
+// end included); 32 rows 3.7 us, the launch and two reads that wait for each other.
 template <int HD, int GS>
 __global__ void __launch_bounds__(256) k_cache_grava(const int8_t* __restrict__ qm, const int8_t* __restrict__ qE, int8_t* __restrict__ cm,
                                                      int8_t* __restrict__ cE, atc::Lote L, int H, int Hk, int lgblk, long long pag_m,
@@ -121,7 +122,8 @@ __global__ void __launch_bounds__(256) k_cache_grava(const int8_t* __restrict__ 
 }
 
 // Whole pages copied, up to PARES_COPIA pairs by value in the launch's arguments (nothing to upload, and a captured graph
-// keeps them). The pairs' targets are distinct and no pair's source, which the host has checked.
+// keeps them). The pairs' targets are distinct and no pair's source, which the host has checked. Bound by its bytes: 300 pages
+// of 12 layers (811 KB each) 92 us, 5.3 TB/s, what a large copy reaches.
 constexpr int PARES_COPIA = 256;
 struct ParesCopia { int de[PARES_COPIA], para[PARES_COPIA]; };
 __global__ void __launch_bounds__(256) k_cache_copia(int8_t* __restrict__ cm, int8_t* __restrict__ cE, ParesCopia ps, long long pag_m, long long pag_e) {
@@ -460,9 +462,9 @@ struct Corrente {
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] = f4_t{0, 0, 0, 0};
     }
-    // weights of a row's scores s (4 keys of every 16 in a lane) as three bf16 pieces, 24 bits, exactly
+    // the maximum raised to a tile's scores s (4 keys of every 16 in a lane); returns what weights take off
     template <int N>
-    __device__ __forceinline__ void pesos(const float (&s)[N], i4_t (&p)[3][N / 8], float K = LOG2E) {
+    __device__ __forceinline__ float sobe(const float (&s)[N], float K = LOG2E) {
         float mx = s[0];
 #pragma unroll
         for (int k = 1; k < N; k++) mx = fmaxf(mx, s[k]);
@@ -475,9 +477,12 @@ struct Corrente {
 #pragma unroll
             for (int d = 0; d < DT; d++) o[d] *= al;
         }
-        const float mL = m == -INFINITY ? 0.f : vezes(m, K);
+        return m == -INFINITY ? 0.f : vezes(m, K);
+    }
+    // weights of 8 scores as three bf16 pieces, 24 bits, exactly
+    __device__ __forceinline__ void pesos(const float* s, i4_t (&p)[3], float mL, float K = LOG2E) {
 #pragma unroll
-        for (int k = 0; k < N; k += 2) {
+        for (int k = 0; k < 8; k += 2) {
             int y[3][2];
 #pragma unroll
             for (int x = 0; x < 2; x++) {
@@ -489,7 +494,7 @@ struct Corrente {
                 y[2][x] = __float_as_int(e1 - __int_as_float(y[1][x] & 0xffff0000));
             }
 #pragma unroll
-            for (int x = 0; x < 3; x++) p[x][k / 8][k % 8 / 2] = (int)__builtin_amdgcn_perm((unsigned)y[x][1], (unsigned)y[x][0], 0x07060302u);
+            for (int x = 0; x < 3; x++) p[x][k / 2] = (int)__builtin_amdgcn_perm((unsigned)y[x][1], (unsigned)y[x][0], 0x07060302u);
         }
     }
     __device__ __forceinline__ void soma_l() {
@@ -549,9 +554,9 @@ struct Corrente {
     }
 };
 
-// O^T += V^T P^T over 32 keys, whose values are the rows of v in LDS (VS bf16 each); p[.][kk]: their weights
-template <int HD, int VS, int N>
-__device__ __forceinline__ void soma_v(Corrente<HD>& y, const __bf16* v, const i4_t (&p)[3][N], int kk, int lr, int c) {
+// O^T += V^T P^T over 32 keys, whose values are the rows of v in LDS (VS bf16 each) and whose weights are p
+template <int HD, int VS>
+__device__ __forceinline__ void soma_v(Corrente<HD>& y, const __bf16* v, const i4_t (&p)[3], int lr, int c) {
     typedef __attribute__((address_space(3))) s4_t* lds4;
     constexpr int DT = Corrente<HD>::DT, DB = DT < 4 ? DT : 4;        // four tiles of dimensions at a time: products in a row do not wait for one another
 #pragma unroll
@@ -567,7 +572,7 @@ __device__ __forceinline__ void soma_v(Corrente<HD>& y, const __bf16* v, const i
 #pragma unroll
         for (int k = 0; k < 3; k++)
 #pragma unroll
-            for (int d = 0; d < DB; d++) y.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[d], __builtin_bit_cast(b8_t, p[k][kk]), y.o[d0 + d], 0, 0, 0);
+            for (int d = 0; d < DB; d++) y.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[d], __builtin_bit_cast(b8_t, p[k]), y.o[d0 + d], 0, 0, 0);
     }
     pronto(y.o);
 }
@@ -767,17 +772,22 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
 // Many rows that share keys and values (new tokens of a sequence, query heads of a group): 16 a wave, 64 per workgroup, on
 // matrix cores; the workgroup walks its keys in tiles of 64. Row rho of a (sequence, kv head) is token rho / Gq,
 // head rho % Gq of the group.
+//   What bounds it is the VALU (0.84 busy): some 440 instructions per wave and tile of 16 rows x 64 keys, of which the weights' powers,
+// sums and pieces are 140, the scores and their maximum 60, the tile's staging 90. 8 prompts of 1 to 4000 tokens, 8 heads of 64:
+// 187 us with the join and the output's values, 250 TFLOP/s; their matrix products alone 39 us. Heads of up to 64 fit four waves a SIMD
+// (128 registers): the pieces of 32 keys are made and used before the next 32's (three waves, all 64 keys' pieces at once: 193 us).
+// Weights summed by matrix products with ones instead of additions: 192 us.
 //   S^T = K Q^T by bf16 MFMA on the values m 2^E themselves, exact in bf16 (8 bits), sums in fp32: a lane holds one row (lane %
 //   16) and 4 keys of each 16, so maxima and sums are in-lane but for two exchanges, and P^T is the next product's
 //   operand as it stands. (i8 MFMA, exact, costs a conversion and two products per score and exponent group: 281 us for
-//   the prompts below.)
+//   these prompts, 210 this way.)
 //   O^T = V^T P^T by bf16 MFMA: P is three bf16 pieces, exact (one piece would leave 2^-8 of every weight, two 2^-16). V^T
 //   comes from row-major LDS by transposing reads.
 // Keys and values are staged once per workgroup, two tiles in LDS: the next tile's loads are in flight while this one is
 // computed, its page numbers one tile earlier still. Slots no row sees are staged as zeros, whatever they hold. The running maximum is
 // raised (and O rescaled) only where a tile exceeds it by 5 nats: weights are then at most e^5, which costs fp32 no precision.
 template <int HD, int GS>
-__global__ void __launch_bounds__(256) k_atc_mf(atc::Args a) {
+__global__ void __launch_bounds__(256, HD <= 64 ? 4 : 2) k_atc_mf(atc::Args a) {
     using namespace atc;
     constexpr int VB = HD < 16 ? HD : 16, LPK = HD / VB, G = HD / GS, TK = 64, NM = HD < 32 ? 1 : HD / 32, RW = 64;
     constexpr int VS = 16 * Corrente<HD>::DT + 8;                     // LDS rows, in values; keys and values alike
@@ -888,10 +898,13 @@ __global__ void __launch_bounds__(256) k_atc_mf(atc::Args a) {
                     s[k] = (j <= i) & ((i - j < janela) | (j < a.sumid)) ? s[k] : -INFINITY;
                 }
             }
-            i4_t p[3][2];
-            y.pesos(s, p, K);
+            const float mL = y.sobe(s, K);
 #pragma unroll
-            for (int kk = 0; kk < 2; kk++) soma_v<HD, VS>(y, &sv[buf][32 * kk * VS], p, kk, lr, c);
+            for (int kk = 0; kk < 2; kk++) {
+                i4_t p[3];
+                y.pesos(s + 8 * kk, p, mL, K);
+                soma_v<HD, VS>(y, &sv[buf][32 * kk * VS], p, lr, c);
+            }
         }
         if (t + 1 < tl.t1) guarda(buf ^ 1);
         __syncthreads();
@@ -906,7 +919,9 @@ __global__ void __launch_bounds__(256) k_atc_mf(atc::Args a) {
 // Up to 16 rows that share keys and values (a new token's query heads of a group, a few new tokens): the same products, but the
 // four waves of a workgroup take every fourth tile of 32 keys for the same rows, without a barrier. A wave reads its keys
 // from memory in the MFMA's own layout, passes its values through its own LDS to transpose them, and has the next
-// tile's bytes in flight while it computes this one. The waves' results are joined at the end. Reading the keys bounds it.
+// tile's bytes in flight while it computes this one. The waves' results are joined at the end.
+// Reading the keys and values bounds it, at 2 waves per SIMD (176 registers; held to 168, which would make them 3, it spills: 155 us): 64
+// sequences of 500 to 4096 tokens, 32 query heads on 8 of 128, 88 us, 3.5 TB/s; 126 us with loads issued when they are needed.
 template <int HD, int GS>
 __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
     using namespace atc;
@@ -1004,9 +1019,9 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
 #pragma unroll
             for (int k = 0; k < 8; k++) s[k] = q.ve(a, j0 + 16 * (k / 4) + 4 * c + k % 4) ? s[k] : -INFINITY;
         }
-        i4_t p[3][1];
-        y.pesos(s, p);
-        soma_v<HD, VS>(y, sv, p, 0, lr, c);
+        i4_t p[3];
+        y.pesos(s, p, y.sobe(s));
+        soma_v<HD, VS>(y, sv, p, lr, c);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     relata_pagina(a, b, ruim);
@@ -1039,7 +1054,8 @@ __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
 
 // ---------------------------------------------------------------------------------------------- values
 // A block or raw tensor as floats (the inverse of de_f32), each value rounded once: block values are exact in both types
-// (8 bits), raw ones are scaled in double precision and rounded to fp32. 8 values a lane; bound by its bytes.
+// (8 bits), raw ones are scaled in double precision and rounded to fp32. 8 values a lane; bound by its bytes: 16,000 x 512 to
+// bf16 5.3 us, 4.7 TB/s.
 template <int TIPO>
 __global__ void __launch_bounds__(256) k_valores(const int8_t* __restrict__ m, const int8_t* __restrict__ E, void* __restrict__ out, long long n, int lgblk) {
     const long long o = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
