@@ -920,7 +920,7 @@ __global__ void __launch_bounds__(256, HD <= 64 ? 4 : 2) k_atc_mf(atc::Args a) {
 // four waves of a workgroup take every fourth tile of 32 keys for the same rows, without a barrier. A wave reads its keys
 // from memory in the MFMA's own layout, passes its values through its own LDS to transpose them, and has the next
 // tile's bytes in flight while it computes this one. The waves' results are joined at the end.
-// Reading the keys and values bounds it, at 2 waves per SIMD (176 registers; held to 168, which would make them 3, it spills: 155 us): 64
+// Reading the keys and values bounds it, at 2 waves per SIMD (196 registers; held to 168, which would make them 3, it spills: 155 us): 64
 // sequences of 500 to 4096 tokens, 32 query heads on 8 of 128, 88 us, 3.5 TB/s; 126 us with loads issued when they are needed.
 template <int HD, int GS>
 __global__ void __launch_bounds__(256) k_atc_gr(atc::Args a) {
