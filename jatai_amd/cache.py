@@ -19,6 +19,9 @@ class CacheKV:
         """paginas pages of `pagina` slots for `camadas` layers of `cabecas` heads of width hd; up to `seqs` sequences of
         max_tokens tokens each."""
         self.ops, self.reg, self.pagina, self.max_tokens = ops, ops.reg, pagina, max_tokens
+        self.reg.exige(min(camadas, cabecas, paginas, seqs, max_tokens) > 0 and hd in (4, 16, 32, 64, 128) and pagina in (16, 32, 64, 128, 256, 512, 1024),
+                       f"CacheKV: {camadas} camadas, {cabecas} cabecas de {hd} (4, 16, 32, 64 ou 128), {paginas} paginas de {pagina} (potencia de 2 de 16 a 1024), "
+                       f"{seqs} sequencias de {max_tokens} tokens")
         P = -(-max_tokens // pagina)
         self.C = (torch.zeros(paginas, camadas, 2, cabecas, pagina, hd, dtype=torch.int8, device=dev),
                   torch.zeros(paginas, camadas, 2, cabecas, pagina, hd // min(hd, O.BLK), dtype=torch.int8, device=dev))

@@ -716,7 +716,7 @@ class OpsHip:
         f = m.shape
         if not (m.dtype == torch.int8 and E.dtype == torch.int8 and m.is_cuda and E.is_cuda and m.dim() == 6 and m.is_contiguous()
                 and E.is_contiguous() and f[2] == 2 and f[5] in (4, 16, 32, 64, 128) and f[4] in (16, 32, 64, 128, 256, 512, 1024)
-                and E.shape == (*f[:5], f[5] // min(f[5], BLK)) and m.numel() and m.get_device() == torch.cuda.current_device()):
+                and E.shape == (*f[:5], f[5] // min(f[5], BLK)) and m.numel() and m.get_device() == E.get_device() == torch.cuda.current_device()):
             self.reg.falha(f"{op}: cache {tuple(f)} {m.dtype} / {tuple(E.shape)} {E.dtype}: esperados int8 contiguos [paginas, camadas, 2, Hk, "
                            f"pagina, hd] e [.., hd / min(hd, {BLK})] na GPU atual, pagina potencia de 2 de 16 a 1024, hd 4, 16, 32, 64 ou 128")
         return f
@@ -727,7 +727,7 @@ class OpsHip:
         self.reg.confere_bloco("qkv", QKV)
         m = QKV[0]
         H = m.shape[1] // hd - 2 * Hk
-        if not (m.shape[1] == (H + 2 * Hk) * hd and H > 0 and H % Hk == 0 and 0 <= camada < camadas and m.get_device() == C[0].get_device()):
+        if not (m.shape[1] == (H + 2 * Hk) * hd and H > 0 and H % Hk == 0 and 0 <= camada < camadas and m.get_device() == QKV[1].get_device() == C[0].get_device()):
             self.reg.falha(f"{op}: qkv {tuple(m.shape)}, camada {camada} de {camadas}, {Hk} cabecas de {hd} no cache")
         tab, comp, ini = lote.tabela, lote.comp, lote.ini
         B = comp.shape[0] if comp.dim() == 1 else -1
@@ -743,7 +743,7 @@ class OpsHip:
     def cache_grava(self, QKV, C, camada, lote):
         """The keys and values of every new row of the block tensor QKV [M, (H + 2 Hk) hd] into the slots of their
         positions, in place; returns C. Rows that belong to no sequence write nothing. Two sequences of a call must not
-        share the pages that they write."""
+        share the pages that they write, nor a sequence name one of them twice."""
         paginas, camadas, Hk, hd, pag, H, B, P = self._confere_lote("cache_grava", QKV, C, camada, lote)
         M = QKV[0].shape[0]
         self._lanca("cache_grava", "jt_cache_grava", (*QKV, *C, paginas, camadas, camada, Hk, hd, pag, lote.tabela, lote.comp, lote.ini, M, B, P,
@@ -801,8 +801,8 @@ class OpsHip:
         m, E = X
         cru = m.dtype == torch.int32
         (self.reg.confere_cru if cru else self.reg.confere_bloco)("x", X)
-        if not (tipo == torch.float32 or (tipo == torch.bfloat16 and not cru)):
-            self.reg.falha(f"valores: tipo {tipo} (float32; bfloat16 para tensores em blocos)")
+        if not ((tipo == torch.float32 or (tipo == torch.bfloat16 and not cru)) and m.get_device() == E.get_device() == torch.cuda.current_device()):
+            self.reg.falha(f"valores: tipo {tipo} (float32; bfloat16 para tensores em blocos), dispositivos {m.device} e {E.device} (a GPU atual)")
         y = torch.empty(m.shape, dtype=tipo, device=m.device)
         self._lanca("valores", "jt_valores", (m, E, y, m.numel(), int(cru), 1 if tipo == torch.bfloat16 else 2), dict(m=m, E=E), tuple(m.shape), longos=(3,))
         return y
@@ -815,7 +815,8 @@ class OpsHip:
         self.reg.confere_bloco("W", W)
         m, E = W
         N, K = m.shape
-        self.reg.exige(0 < K <= 256 * BLK and N > 0, f"para4: N={N}, K={K} (K ate {256 * BLK})")
+        self.reg.exige(0 < K <= 256 * BLK and N > 0 and m.get_device() == E.get_device() == torch.cuda.current_device(),
+                       f"para4: N={N}, K={K} (K ate {256 * BLK}), dispositivos {m.device} e {E.device} (a GPU atual)")
         Nt, Kt = -(-N // 16), -(-K // 128)
         P = (torch.empty(Nt, Kt, 64, 16, dtype=torch.uint8, device=m.device),
              torch.empty(Nt, Kt, 16, 128 // BLK, dtype=torch.bfloat16, device=m.device), torch.empty(N, dtype=torch.int16, device=m.device))
@@ -829,14 +830,15 @@ class OpsHip:
         Nt, Kt = -(-N // 16), -(-K // 128)
         if not (w.dtype == torch.uint8 and esc.dtype == torch.bfloat16 and r.dtype == torch.int16 and w.shape == (Nt, Kt, 64, 16)
                 and esc.shape == (Nt, Kt, 16, 128 // BLK) and r.dim() == 1 and w.is_contiguous() and esc.is_contiguous() and r.is_contiguous()
-                and 0 < K <= 256 * BLK and N > 0 and (modo == 1 or N % BLK == 0) and x.get_device() == w.get_device() == esc.get_device() == r.get_device()):
+                and 0 < K <= 256 * BLK and N > 0 and (modo == 1 or N % BLK == 0)
+                and x.get_device() == xE.get_device() == w.get_device() == esc.get_device() == r.get_device() == torch.cuda.current_device()):
             self.reg.falha(f"{op}: X {tuple(x.shape)}, pesos {tuple(w.shape)} {w.dtype}, escalas {tuple(esc.shape)} {esc.dtype}, expoentes "
-                           f"{tuple(r.shape)} {r.dtype} (de para4, com BLK={BLK}, K ate {256 * BLK}; N multiplo de {BLK}, ou cru)")
+                           f"{tuple(r.shape)} {r.dtype} (de para4, com BLK={BLK}, K ate {256 * BLK}; N multiplo de {BLK}, ou cru), todos na GPU atual")
         ent = dict(X=x, XE=xE, W=w, escalas=esc, R=r)
         if R is not None:
             self.reg.confere_bloco("R", R)
-            if R[0].shape != (M, N):
-                self.reg.falha(f"{op}: R com forma {tuple(R[0].shape)}, esperado {(M, N)}")
+            if not (R[0].shape == (M, N) and R[0].get_device() == R[1].get_device() == x.get_device()):
+                self.reg.falha(f"{op}: R com forma {tuple(R[0].shape)}, esperado {(M, N)} na GPU de X")
             ent.update(res=R[0], resE=R[1])
         if modo == 1:
             Y = (torch.empty(M, N, dtype=torch.int32, device=x.device), torch.empty(M, N, dtype=torch.int16, device=x.device))

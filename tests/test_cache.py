@@ -217,3 +217,54 @@ def test_guardas_python_sem_gpu(tmp_path, monkeypatch):
     W64 = (z(4, 2, 64, 16, tipo=torch.uint8), z(4, 2, 16, 4, tipo=torch.bfloat16), z(64, tipo=torch.int16))
     with pytest.raises(ErroJatai):
         ops.gemv4_soma(X, W64, (z(5, 96), z(5, 3)))
+
+
+def test_recusas_de_construcao(tmp_path):
+    ops = OpsFalso(tmp_path, 4)
+    for a in ((0, 2, 16, 4, 2, 32, 16), (1, 0, 16, 4, 2, 32, 16), (1, 2, 8, 4, 2, 32, 16), (1, 2, 16, 0, 2, 32, 16), (1, 2, 16, 4, 0, 32, 16), (1, 2, 16, 4, 2, 0, 16),
+              (1, 2, 16, 4, 2, 32, 24), (1, 2, 16, 4, 2, 32, 8), (1, 2, 16, 4, 2, 32, 2048)):
+        with pytest.raises(ErroJatai, match="CacheKV"):
+            CacheKV(ops, *a, dev="cpu")
+
+
+def test_outro_dispositivo(tmp_path, monkeypatch):
+    """Operands that lie on different GPUs, or on another than the current one, are refused before anything is launched."""
+    class NaGpu(torch.Tensor):
+        is_cuda = property(lambda self: True)
+        dispositivo = 0
+
+        def get_device(self):
+            return self.dispositivo
+
+    def z(*forma, tipo=torch.int8, d=0):
+        t = torch.zeros(*forma, dtype=tipo).as_subclass(NaGpu)
+        t.dispositivo = d
+        return t
+    atual = [0]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: atual[0])
+    monkeypatch.setattr(O, "BLK", 32)
+    ops = object.__new__(O.OpsHip)
+    ops.reg, ops._blk, lancados = Registro(str(tmp_path), "g", eco=False), 32, []
+    ops._lanca = lambda op, *a, **k: lancados.append(op)
+    bf, i16, i32 = torch.bfloat16, torch.int16, torch.int32
+    usos = [(lambda m, E: ops.valores((m, E)), [(z, (4, 64)), (z, (4, 2))]),
+            (lambda a, e: ops.valores((a, e)), [(lambda *f, d=0: z(*f, tipo=i32, d=d), (4, 64)), (lambda *f, d=0: z(*f, tipo=i16, d=d), (4, 64))]),
+            (lambda m, E: ops.para4((m, E)), [(z, (32, 128)), (z, (32, 4))]),
+            (lambda x, xE, w, s, r, m, E: ops.gemv4_soma((x, xE), (w, s, r), (m, E)),
+             [(z, (3, 128)), (z, (3, 4)), (lambda *f, d=0: z(*f, tipo=torch.uint8, d=d), (2, 1, 64, 16)), (lambda *f, d=0: z(*f, tipo=bf, d=d), (2, 1, 16, 4)),
+              (lambda *f, d=0: z(*f, tipo=i16, d=d), (32,)), (z, (3, 32)), (z, (3, 1))]),
+            (lambda m, E, cm, cE, t, c: ops.cache_grava((m, E), (cm, cE), 0, O.Lote(t, c, None, 1, 16)),
+             [(z, (4, 384)), (z, (4, 12)), (z, (6, 1, 2, 2, 16, 64)), (z, (6, 1, 2, 2, 16, 2)), (lambda *f, d=0: z(*f, tipo=i32, d=d), (2, 1)),
+              (lambda *f, d=0: z(*f, tipo=i32, d=d), (2,))])]
+    for f, partes in usos:
+        lancados.clear()
+        f(*(g(*forma) for g, forma in partes))
+        assert len(lancados) == 1
+        for k in range(len(partes)):
+            with pytest.raises(ErroJatai):
+                f(*(g(*forma, d=int(i == k)) for i, (g, forma) in enumerate(partes)))
+        atual[0] = 1
+        with pytest.raises(ErroJatai):
+            f(*(g(*forma) for g, forma in partes))
+        atual[0] = 0
+        assert len(lancados) == 1
