@@ -7,10 +7,16 @@ attention is `OpsHip.atencao_cache`, softmax in float32 over exact products, wit
 Where the training attention aligns a whole window to one exponent and rounds its weights to 8 bits, this one rounds
 only its output, so that a token's result does not depend on what comes later and lengths are not bound to 512.
 """
+import weakref
+
 import torch
 
 from . import ops as O
 from .cache import CacheKV
+
+# generators with steps whose device events have not been read: the device holds one record for all, which is cleared only when
+# nobody has any left to read
+_pendentes = weakref.WeakSet()
 
 
 class Gerador:
@@ -32,7 +38,6 @@ class Gerador:
         self.tok, self.vivas, self.comp, self._grafo, self.lancamentos = z(self.linhas), z(seqs), z(seqs), None, []
         self._indices = torch.arange(modelo.V, dtype=torch.int32, device=modelo.dev)
         self._estado = None                        # (live sequences, their lengths) as the device tensors hold them
-        self._pendente = False                     # steps whose device events have not been read
 
     # ------------------------------------------------------------------ the forward pass of new tokens
     def _produto(self, X, n):
@@ -80,11 +85,13 @@ class Gerador:
 
     def le(self, textos):
         """New tokens for some sequences, textos = {sequence: tokens (at least one)}: prompts, or continuations of what the
-        cache holds. Returns the logits after each one's last token, float32 [len(textos), V] in textos' order."""
+        cache holds. Returns the logits after each one's last token, float32 [len(textos), V] in textos' order. An error leaves
+        the sequences it was called for with nothing of use: free them."""
         reg, V = self.reg, self.m.V
         reg.exige(len(textos) > 0 and all(len(t) > 0 for t in textos.values()), "le: cada sequencia com pelo menos um token")
         reg.exige(all(0 <= x < V for t in textos.values() for x in t), f"le: tokens de 0 a {V - 1}")
-        self.confere()
+        for g in list(_pendentes):
+            g.confere()
         reg.novo_passo(reg.passo)
         self.cache.reserva({s: len(t) for s, t in textos.items()})
         self.cache.envia()
@@ -106,9 +113,10 @@ class Gerador:
         return y
 
     def confere(self):
-        """Reads the device events of the steps so far (waits for them); one that was raised becomes an ErroJatai."""
-        if self._pendente:
-            self._pendente = False
+        """Reads the device events of the steps so far (waits for them); one that was raised becomes an ErroJatai. Comes before
+        training steps or other work that clears the device's record; of several generators with steps to read each one raises."""
+        if self in _pendentes:
+            _pendentes.discard(self)
             self.reg.lancamentos = self.lancamentos
             self.reg.fim_passo()
 
@@ -143,7 +151,7 @@ class Gerador:
         self.reg.exige(len(set(vivas)) == len(vivas), f"passo: sequencia repetida em {vivas}")
         if self._grafo is None:
             self._grava()
-        if not self._pendente:
+        if not _pendentes:
             self.reg.novo_passo(self.reg.passo)
         self.cache.reserva({s: 1 for s in vivas})
         estado = (vivas, [self.cache.n[s] - 1 for s in vivas])
@@ -156,8 +164,9 @@ class Gerador:
         self.cache.envia(comprimentos=False)
         self.tok[:self.seqs].copy_(tok)
         self._grafo.replay()
-        self._estado, self._pendente = (vivas, [n + 1 for n in estado[1]]), True
-        self.reg.lancamentos = self.lancamentos
+        self._estado = (vivas, [n + 1 for n in estado[1]])
+        _pendentes.add(self)
+        self.reg.lancamentos = list(self.lancamentos)
         self._esquece()
         return self.logits, self.escolha
 

@@ -261,3 +261,48 @@ def test_evento_num_passo_gravado():
     with pytest.raises(ErroJatai, match="atencao_cache") as e:
         g.confere()
     assert "passo / camada 0 / atencao" in str(e.value) and "valor    : 1000000" in str(e.value)
+
+
+def test_evento_de_um_entre_dois_geradores():
+    """The device has one event record: another generator's steps and prompts do not clear what one has yet to read."""
+    from jatai_amd.registro import ErroJatai
+    tok = torch.zeros(3, dtype=torch.int32, device="cuda")
+    for depois in ("passo", "le"):
+        a, b = _gerador(_modelo("cab64")), _gerador(_modelo("cab64"))
+        for g in (a, b):
+            g.le({0: _texto(1, 20)})
+            g.passo([0], tok)
+            g.confere()
+        a.cache.tabela[0, 0] = 10**6
+        a.passo([0], tok)
+        if depois == "passo":
+            b.passo([0], tok)
+            with pytest.raises(ErroJatai, match="invalid argument"):
+                a.confere()
+            with pytest.raises(ErroJatai):
+                b.confere()
+        else:
+            with pytest.raises(ErroJatai, match="invalid argument"):
+                b.le({1: _texto(2, 5)})
+        b.le({2: _texto(3, 5)})                                        # the record is cleared once everyone has read it
+        b.passo([0], tok)
+        b.confere()
+
+
+def test_desalinhados():
+    """Contiguous tensors that do not begin at 16 bytes are refused; nothing is written."""
+    from backends import GPU
+    from jatai_amd.registro import ErroJatai
+    g = GPU(32)
+    torto = lambda *f: torch.zeros(int(torch.Size(f).numel()) + 8, dtype=torch.int8, device="cuda")[3:-5].view(f)
+    reto = lambda *f: torch.zeros(f, dtype=torch.int8, device="cuda")
+    i32 = lambda *f: torch.zeros(f, dtype=torch.int32, device="cuda")
+    lote = g.O.Lote(i32(2, 1), i32(2), None, 1, 16)
+    qkv, C = (lambda m: (m, reto(4, 12))), (lambda m: (m, reto(6, 1, 2, 2, 16, 2)))
+    X, P = (lambda m: (m, reto(3, 4))), g.ops.para4((reto(32, 128), reto(32, 4)))
+    for f in (lambda: g.ops.cache_grava(qkv(torto(4, 384)), C(reto(6, 1, 2, 2, 16, 64)), 0, lote), lambda: g.ops.cache_grava(qkv(reto(4, 384)), C(torto(6, 1, 2, 2, 16, 64)), 0, lote),
+              lambda: g.ops.atencao_cache(qkv(torto(4, 384)), C(reto(6, 1, 2, 2, 16, 64)), 0, lote), lambda: g.ops.cache_copia(C(torto(6, 1, 2, 2, 16, 64)), [(0, 1)]),
+              lambda: g.ops.gemv4(X(torto(3, 128)), P), lambda: g.ops.para4((torto(32, 128), reto(32, 4))), lambda: g.ops.valores(X(torto(3, 128)))):
+        with pytest.raises(ErroJatai, match="refused the launch"):
+            f()
+    g.reg.fim_passo()
