@@ -772,9 +772,9 @@ __global__ void __launch_bounds__(256) k_atc_um(atc::Args a) {
 // Many rows that share keys and values (new tokens of a sequence, query heads of a group): 16 a wave, 64 per workgroup, on
 // matrix cores; the workgroup walks its keys in tiles of 64. Row rho of a (sequence, kv head) is token rho / Gq,
 // head rho % Gq of the group.
-//   What bounds it is the VALU (0.84 busy): some 440 instructions per wave and tile of 16 rows x 64 keys, of which the weights' powers,
+//   What bounds it is the VALU (0.94 busy): some 440 instructions per wave and tile of 16 rows x 64 keys, of which the weights' powers,
 // sums and pieces are 140, the scores and their maximum 60, the tile's staging 90. 8 prompts of 1 to 4000 tokens, 8 heads of 64:
-// 187 us with the join and the output's values, 250 TFLOP/s; their matrix products alone 39 us. Heads of up to 64 fit four waves a SIMD
+// 184 us with the join and the output's values, 254 TFLOP/s; their matrix products alone 39 us. Heads of up to 64 fit four waves a SIMD
 // (128 registers): the pieces of 32 keys are made and used before the next 32's (three waves, all 64 keys' pieces at once: 193 us).
 // Weights summed by matrix products with ones instead of additions: 192 us.
 //   S^T = K Q^T by bf16 MFMA on the values m 2^E themselves, exact in bf16 (8 bits), sums in fp32: a lane holds one row (lane %
