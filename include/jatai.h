@@ -202,7 +202,8 @@ int jt_cache_grava(const void* qm, const void* qE, void* cm, void* cE, int npag,
 int jt_cache_copia(void* cm, void* cE, int npag, int camadas, int Hk, int hd, int pag, const void* pares, int n, int kid);
 /* out [M, H hd]: softmax_j(q . k_j / sqrt(hd) - incl[h] (i - j)) . v_j over the visible tokens j <= i of the row's sequence:
  * all (janela 0), or the last janela and the first sumid. Query head h reads head h / (H / Hk); incl float [H] or null.
- * tipo 0: block tensor (out int8, outE), 1: bfloat16, 2: fp32. Rows of no sequence come out as zeros. ws: workspace of
+ * tipo 0: block tensor (out int8, outE), 1: bfloat16, 2: fp32. Rows of no sequence come out as zeros; scores
+ * beyond fp32 give NaN, or E_EXP in a block output. ws: workspace of
  * jt_atencao_cache_ws_bytes bytes (0: none, ws may be null; it depends on the block size), 16-byte aligned, not shared by calls that overlap. */
 long long jt_atencao_cache_ws_bytes(int M, int B, int H, int Hk, int hd, int novos, int teto, int janela, int sumid, int tipo);
 int jt_atencao_cache(const void* qm, const void* qE, const void* cm, const void* cE, int npag, int camadas, int camada, int Hk, int hd, int pag,
