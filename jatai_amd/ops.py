@@ -11,7 +11,9 @@ ops.py:17), E_ZERO, GA, ATENCAO_LIMITE (attention-backward bound variant, ops.py
 
 There is no CPU fallback: if libjatai.so is missing or fails to load, constructing OpsHip raises.
 """
+import array
 import ctypes
+import itertools
 import math
 import os
 import typing
@@ -754,10 +756,10 @@ class OpsHip:
         """Pages copied within the cache, every layer of them, in place; returns C. pares: [(source, target)], the targets
         distinct and none of them a source."""
         paginas, camadas, _, Hk, pag, hd = self._confere_cache("cache_copia", C)
-        v = [p for par in pares for p in par]
-        if not (len(v) == 2 * len(pares) and all(0 <= p < paginas for p in v) and len({*v[1::2]}) == len(pares) and not {*v[1::2]} & {*v[::2]}):
+        v = list(itertools.chain.from_iterable(pares))
+        if not (len(v) == 2 * len(pares) and (not v or 0 <= min(v) <= max(v) < paginas) and len({*v[1::2]}) == len(pares) and not {*v[1::2]} & {*v[::2]}):
             self.reg.falha(f"cache_copia: pares (origem, destino) de paginas 0 a {paginas - 1}, destinos distintos e nenhum deles origem; recebeu {pares}")
-        tab = (ctypes.c_int * len(v))(*v)
+        tab = (ctypes.c_int * len(v)).from_buffer(array.array("i", v))
         self._lanca("cache_copia", "jt_cache_copia", (*C, paginas, camadas, Hk, hd, pag, tab, len(pares)), dict(), (len(pares),))
         return C
 
